@@ -275,7 +275,7 @@ def prepare(case, seed):
         if case["op"] == "sample":
             s["handle"] = eii.Sampler(torch.cuda.current_device())
         else:
-            rope = s["rope"] if case["op"] == "append" else None
+            rope = s["rope"] if case["op"] == "append" else _rope(512, case["hd"])
             s["handle"] = eii.Paged(case["heads"], case["kv"], case["hd"], case["page"], case["bits"], rope=rope,
                                     device=torch.cuda.current_device())
             s["pages"] = eii.Pages(s["k_pool"].data_ptr(), s["v_pool"].data_ptr(), s["k_pool"].shape[0],
