@@ -71,6 +71,18 @@ _SIGS = {
                               ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
     "eii_linear_plan_run": ([_P, _P, ctypes.c_int, _P, ctypes.c_int64, _P, _P, _P], ctypes.c_int),
     "eii_linear_plan_close": ([_P], None),
+    "eii_paged_open": ([ctypes.c_int] * 7 + [_P, _P, ctypes.POINTER(_P)], ctypes.c_int),
+    "eii_paged_pool_bytes": ([_P, ctypes.c_int64], ctypes.c_int64),
+    "eii_paged_append": ([_P, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+                          _P, _P, ctypes.c_int, ctypes.c_int, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
+    "eii_paged_attention": ([_P, _P, _P, ctypes.c_int64, ctypes.c_int, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                             ctypes.c_int, ctypes.c_int, _P, ctypes.c_int64, _P], ctypes.c_int),
+    "eii_paged_sync": ([_P, _P], ctypes.c_int),
+    "eii_paged_close": ([_P], None),
+    "eii_sampler_open": ([ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
+    "eii_sample": ([_P, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int] + [_P] * 9, ctypes.c_int),
+    "eii_sampler_sync": ([_P, _P], ctypes.c_int),
+    "eii_sampler_close": ([_P], None),
 }
 
 
@@ -387,6 +399,98 @@ class Decoder:
 
     def sync(self, stream=None):
         check(lib().eii_decoder_sync(self.h, ctypes.c_void_p(stream) if stream else None))
+
+
+class Pages(ctypes.Structure):
+    """eii_pages of include/eii.h: one layer's pools and page table, as device pointers."""
+    _fields_ = [("k_pool", _P), ("v_pool", _P), ("n_pages", ctypes.c_int64), ("table", _P), ("ld_table", ctypes.c_int64),
+                ("n_seq", ctypes.c_int)]
+
+
+class Paged:
+    """Paged K/V cache of 16 or 4 bits (include/eii.h, eii_paged_*).  Pointers are device pointers on
+    `device`; strides are in elements and default to dense rows.  The calls enqueue on `stream` (None:
+    the legacy default stream) and return; sync() reports device-side errors."""
+
+    def __init__(self, n_heads, n_kv, head_dim, page_size, cache_bits, n_pos=512, rope=None, device=0):
+        """rope: (cos, sin) Q30 tables [n_pos, head_dim / 2], which then give n_pos; None (head_dim 64
+        only) generates the model's own for n_pos positions."""
+        self.h = None
+        c = s = None
+        if rope is not None:
+            c, s = _c(rope[0], np.int64), _c(rope[1], np.int64)
+            if c.ndim != 2 or c.shape != s.shape or c.shape[1] != head_dim // 2:
+                raise EiiError(EII_ERR_ARG, f"rope tables must be [n_pos, {head_dim // 2}], got {c.shape} and {s.shape}")
+            n_pos = c.shape[0]
+        h = ctypes.c_void_p()
+        check(lib().eii_paged_open(int(device), int(n_heads), int(n_kv), int(head_dim), int(page_size), int(cache_bits),
+                                   int(n_pos), ptr(c), ptr(s), ctypes.byref(h)))
+        self.h = h
+        self.device = device
+        self.q_row, self.kv_row = int(n_heads) * int(head_dim), int(n_kv) * int(head_dim)
+
+    def close(self):
+        if self.h:
+            lib().eii_paged_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def pool_bytes(self, n_pages):
+        n = lib().eii_paged_pool_bytes(self.h, int(n_pages))
+        if n < 0:
+            check(-n)
+        return n
+
+    def append(self, pages, k_ptr, v_ptr, n_rows, pos_ptr, shift_k, seq_ptr=None, q_ptr=None, q_out_ptr=None, shift_q=1,
+               in_bits=16, ldq=None, ldk=None, ldv=None, ldqo=None, kv_out_ptr=None, stream=None):
+        check(lib().eii_paged_append(self.h, ctypes.byref(pages), q_ptr, self.q_row if ldq is None else ldq, k_ptr,
+                                     self.kv_row if ldk is None else ldk, v_ptr, self.kv_row if ldv is None else ldv,
+                                     int(in_bits), int(n_rows), seq_ptr, pos_ptr, int(shift_q), int(shift_k), q_out_ptr,
+                                     self.q_row if ldqo is None else ldqo, kv_out_ptr, stream))
+
+    def attention(self, pages, q_ptr, n_rows, len_ptr, max_len, shift_s, shift_c, bits_c, out_ptr, seq_ptr=None,
+                  prob_bits=16, ldq=None, ldc=None, stream=None):
+        check(lib().eii_paged_attention(self.h, ctypes.byref(pages), q_ptr, self.q_row if ldq is None else ldq,
+                                        int(n_rows), seq_ptr, len_ptr, int(max_len), int(shift_s), int(prob_bits),
+                                        int(shift_c), int(bits_c), out_ptr, self.q_row if ldc is None else ldc, stream))
+
+    def sync(self, stream=None):
+        check(lib().eii_paged_sync(self.h, stream))
+
+
+class Sampler:
+    """Token draws from int32 logits and given random words (include/eii.h, eii_sample).  Device
+    pointers; the call enqueues on `stream` (None: the legacy default stream) and returns."""
+
+    def __init__(self, device=0):
+        self.h = None
+        h = ctypes.c_void_p()
+        check(lib().eii_sampler_open(int(device), ctypes.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h:
+            lib().eii_sampler_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def sample(self, logits_ptr, n_rows, vocab, u_ptr, token_ptr, ld=None, inv_temp_ptr=None, top_k_ptr=None,
+               top_p_ptr=None, min_p_ptr=None, kept_ptr=None, prob_ptr=None, stream=None):
+        check(lib().eii_sample(self.h, logits_ptr, vocab if ld is None else ld, int(n_rows), int(vocab), inv_temp_ptr,
+                               top_k_ptr, top_p_ptr, min_p_ptr, u_ptr, token_ptr, kept_ptr, prob_ptr, stream))
+
+    def sync(self, stream=None):
+        check(lib().eii_sampler_sync(self.h, stream))
 
 
 def _mix64(z):

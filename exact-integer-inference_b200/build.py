@@ -16,6 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(HERE, "libeii.so")
 CLI = os.path.join(HERE, "eii_check")
+OBJ = os.path.join(REPO, "_build", "obj")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC = os.environ.get("NVCC", "nvcc")
 
@@ -35,8 +36,22 @@ def _stale(target, deps):
 def build(force=False, verbose=False):
     deps = _sources()
     if force or _stale(LIB, deps):
-        cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-O2",
-               "-I" + INCLUDE, "-I" + CSRC, "-o", LIB, os.path.join(CSRC, "eii_engine.cu")]
+        os.makedirs(OBJ, exist_ok=True)
+        headers = [d for d in deps if not d.endswith((".cu", ".c"))]
+        objs, jobs = [], []
+        for src in (d for d in deps if d.endswith(".cu")):
+            obj = os.path.join(OBJ, os.path.basename(src)[:-3] + ".o")
+            objs.append(obj)
+            if force or _stale(obj, [src, *headers]):
+                cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-I" + INCLUDE,
+                       "-I" + CSRC, "-c", "-o", obj, src]
+                if verbose:
+                    print(" ".join(cmd), flush=True)
+                jobs.append((cmd, subprocess.Popen(cmd)))
+        failed = [cmd for cmd, job in jobs if job.wait() != 0]
+        if failed:
+            raise subprocess.CalledProcessError(1, failed[0])
+        cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objs]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)

@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "eii.h"
+#include "eii_host.h"
 #include "eii_attn.cuh"
 #include "eii_tables.h"
 #include "eii_gemm.cuh"
@@ -41,10 +42,10 @@
 using namespace eii;
 
 namespace {
-
 thread_local std::string g_err;
+}
 
-int fail(int code, const char* fmt, ...) {
+int eii::fail(int code, const char* fmt, ...) {
     char buf[1024];
     va_list ap;
     va_start(ap, fmt);
@@ -54,17 +55,19 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define CK(call)                                                                                      \
-    do {                                                                                              \
-        cudaError_t e_ = (call);                                                                      \
-        if (e_ != cudaSuccess)                                                                        \
-            return fail(EII_ERR_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
-    } while (0)
-#define TRY(...)                         \
-    do {                                 \
-        int rc_ = (__VA_ARGS__);         \
-        if (rc_ != EII_OK) return rc_;   \
-    } while (0)
+int eii::check_device(int device) {
+    int ndev = 0;
+    cudaError_t st = cudaGetDeviceCount(&ndev);
+    if (st != cudaSuccess || ndev == 0) return fail(EII_ERR_CUDA, "no CUDA device (%s)", cudaGetErrorString(st));
+    if (device < 0 || device >= ndev) return fail(EII_ERR_ARG, "device %d out of range [0, %d)", device, ndev);
+    int major = 0, minor = 0;
+    CK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    CK(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+    if (major != 10) return fail(EII_ERR_CUDA, "device %d is sm_%d%d; this build needs sm_100", device, major, minor);
+    return EII_OK;
+}
+
+namespace {
 
 constexpr int MODEL_LIN_N[7] = {576, 192, 192, 576, 1536, 1536, 576};
 constexpr int MODEL_LIN_K[7] = {576, 576, 576, 576, 576, 576, 1536};
@@ -1155,19 +1158,14 @@ int load_model(eii_engine* e, const uint8_t* data, size_t nbytes) {
 int open_common(const void* data, size_t nbytes, int device, eii_engine** out) {
     if (!out) return fail(EII_ERR_ARG, "out is null");
     *out = nullptr;
-    int ndev = 0;
-    cudaError_t st = cudaGetDeviceCount(&ndev);
-    if (st != cudaSuccess || ndev == 0) return fail(EII_ERR_CUDA, "no CUDA device (%s)", cudaGetErrorString(st));
-    if (device < 0 || device >= ndev) return fail(EII_ERR_ARG, "device %d out of range [0, %d)", device, ndev);
+    TRY(check_device(device));
     CK(cudaSetDevice(device));
-    cudaDeviceProp prop;
-    CK(cudaGetDeviceProperties(&prop, device));
-    if (prop.major != 10) return fail(EII_ERR_CUDA, "device %d is sm_%d%d; this build needs sm_100", device, prop.major, prop.minor);
     eii_engine* e = new eii_engine();
     e->device = device;
-    e->num_sms = prop.multiProcessorCount;
     int rc = EII_OK;
-    if (cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking) != cudaSuccess) rc = fail(EII_ERR_CUDA, "stream create failed");
+    if (cudaDeviceGetAttribute(&e->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+        rc = fail(EII_ERR_CUDA, "device attributes unavailable");
+    if (rc == EII_OK && cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking) != cudaSuccess) rc = fail(EII_ERR_CUDA, "stream create failed");
     if (rc == EII_OK) rc = dalloc(e->weights, &e->err_dev, 1);
     if (rc == EII_OK && cudaMemset(e->err_dev, 0, sizeof(int)) != cudaSuccess) rc = fail(EII_ERR_CUDA, "memset failed");
     if (rc == EII_OK) rc = load_model(e, static_cast<const uint8_t*>(data), nbytes);

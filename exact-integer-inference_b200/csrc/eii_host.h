@@ -1,0 +1,42 @@
+// Host-side helpers shared by the translation units of libeii.so: the thread-local error message
+// behind eii_last_error(), the CUDA error check, and a guard for the caller's current device.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "eii.h"
+
+namespace eii {
+
+// Records the message of a failed call on this thread and returns `code`.
+int fail(int code, const char* fmt, ...);
+
+#define CK(call)                                                                                      \
+    do {                                                                                              \
+        cudaError_t e_ = (call);                                                                      \
+        if (e_ != cudaSuccess)                                                                        \
+            return fail(EII_ERR_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
+    } while (0)
+#define TRY(...)                         \
+    do {                                 \
+        int rc_ = (__VA_ARGS__);         \
+        if (rc_ != EII_OK) return rc_;   \
+    } while (0)
+
+// Makes `device` current for a scope and restores the caller's device afterwards.
+struct DeviceGuard {
+    int before = -1;
+    cudaError_t st = cudaSuccess;
+    explicit DeviceGuard(int device) {
+        st = cudaGetDevice(&before);
+        if (st == cudaSuccess && before != device) st = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// `device` exists and is sm_100 (EII_ERR_CUDA / EII_ERR_ARG otherwise); leaves the current device alone.
+int check_device(int device);
+
+}  // namespace eii

@@ -1,0 +1,250 @@
+// C ABI of the paged K/V cache (eii_paged_*): argument checks, handle, launches.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <new>
+#include <vector>
+
+#include "eii.h"
+#include "eii_host.h"
+#include "eii_paged.cuh"
+
+using namespace eii;
+
+struct eii_paged {
+    int device = 0, num_sms = 0;
+    int n_heads = 0, n_kv = 0, hd = 0, page_shift = 0, bits = 0, n_pos = 0;
+    int32_t *exp_tab = nullptr, *rope_c = nullptr, *rope_s = nullptr;
+    int* err = nullptr;
+    uint8_t* mem = nullptr;  // the four above, one allocation
+};
+
+namespace {
+
+int64_t slab_bytes(const eii_paged* p) {
+    return static_cast<int64_t>(paged_row_bytes(p->hd, p->bits)) << p->page_shift;
+}
+
+int check_pages(const eii_paged* p, const eii_pages* pg) {
+    if (!pg) return fail(EII_ERR_ARG, "pages is null");
+    if (!pg->k_pool || !pg->v_pool || !pg->table) return fail(EII_ERR_ARG, "a pool or the page table is null");
+    if ((reinterpret_cast<uintptr_t>(pg->k_pool) | reinterpret_cast<uintptr_t>(pg->v_pool)) & 15)
+        return fail(EII_ERR_ARG, "the pools must be 16-byte aligned");
+    if (pg->n_pages < 1 || pg->n_pages > INT32_MAX)
+        return fail(EII_ERR_ARG, "n_pages must be in [1, 2^31) (got %lld)", (long long)pg->n_pages);
+    if (pg->n_seq < 1) return fail(EII_ERR_ARG, "n_seq must be >= 1 (got %d)", pg->n_seq);
+    if (pg->ld_table < 1) return fail(EII_ERR_ARG, "ld_table must be >= 1 (got %lld)", (long long)pg->ld_table);
+    (void)p;
+    return EII_OK;
+}
+
+PagedGeom geometry(const eii_paged* p, const eii_pages* pg) {
+    PagedGeom g{};
+    g.n_heads = p->n_heads; g.n_kv = p->n_kv; g.hd = p->hd; g.group = p->n_heads / p->n_kv;
+    g.page_shift = p->page_shift; g.bits = p->bits; g.slab = slab_bytes(p);
+    g.k_pool = static_cast<uint8_t*>(pg->k_pool); g.v_pool = static_cast<uint8_t*>(pg->v_pool);
+    g.n_pages = pg->n_pages; g.table = pg->table; g.ld_table = pg->ld_table; g.n_seq = pg->n_seq;
+    g.exp_tab = p->exp_tab; g.err = p->err;
+    return g;
+}
+
+int check_shift(const char* name, int s) {
+    if (s < 1 || s > 62) return fail(EII_ERR_ARG, "%s must be in [1, 62] (got %d)", name, s);
+    return EII_OK;
+}
+
+int check_ld(const char* name, int64_t ld, int64_t least) {
+    if (ld < least) return fail(EII_ERR_ARG, "%s must be >= %lld (got %lld)", name, (long long)least, (long long)ld);
+    return EII_OK;
+}
+
+template <int HD, int BITS>
+int launch_append(const AppendParams& ap, int in_bits, cudaStream_t st) {
+    const int64_t warps = static_cast<int64_t>(ap.n_rows) * ((ap.q ? ap.g.n_heads : 0) + 2 * ap.g.n_kv);
+    const int64_t blocks = (warps + 7) / 8;
+    if (blocks > INT32_MAX) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
+    if (in_bits == 16) k_paged_append<HD, BITS, int16_t><<<(unsigned)blocks, 256, 0, st>>>(ap);
+    else k_paged_append<HD, BITS, int32_t><<<(unsigned)blocks, 256, 0, st>>>(ap);
+    CK(cudaGetLastError());
+    return EII_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_size, int cache_bits, int n_pos,
+                   const int64_t* rope_cos, const int64_t* rope_sin, eii_paged** out) {
+    if (!out) return fail(EII_ERR_ARG, "out is null");
+    *out = nullptr;
+    if (n_heads < 1 || n_kv < 1 || n_heads % n_kv != 0 || n_heads > 1024)
+        return fail(EII_ERR_ARG, "n_heads must be a multiple of n_kv in [1, 1024] (got %d and %d)", n_heads, n_kv);
+    if (head_dim != 64 && head_dim != 128) return fail(EII_ERR_ARG, "head_dim must be 64 or 128 (got %d)", head_dim);
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+        return fail(EII_ERR_ARG, "page_size must be a power of two in [16, 1024] (got %d)", page_size);
+    if (cache_bits != 4 && cache_bits != 16) return fail(EII_ERR_ARG, "cache_bits must be 4 or 16 (got %d)", cache_bits);
+    if (n_pos < 1 || n_pos > EII_PAGED_MAX_LEN)
+        return fail(EII_ERR_ARG, "n_pos must be in [1, %d] (got %d)", EII_PAGED_MAX_LEN, n_pos);
+    if (!rope_cos != !rope_sin) return fail(EII_ERR_ARG, "rope_cos and rope_sin come together");
+    if (!rope_cos && head_dim != 64)
+        return fail(EII_ERR_ARG, "head_dim %d needs rope tables (they are generated for head_dim 64 only)", head_dim);
+    const size_t n = static_cast<size_t>(n_pos) * (head_dim / 2);
+    std::vector<int64_t> e, c, s;
+    std::vector<int32_t> h;
+    try {
+        e.resize(PAGED_DMAX + 1);
+        if (!rope_cos) {
+            c.resize(n);
+            s.resize(n);
+            TRY(eii_table_rope(n_pos, c.data(), s.data()));
+            rope_cos = c.data();
+            rope_sin = s.data();
+        }
+        h.resize(PAGED_DMAX + 1 + 2 * n);
+    } catch (const std::bad_alloc&) {
+        return fail(EII_ERR_ARG, "out of host memory for %d positions", n_pos);
+    }
+    TRY(eii_table_exp(e.data()));
+    for (int i = 0; i <= PAGED_DMAX; ++i) h[i] = static_cast<int32_t>(e[i]);
+    for (size_t i = 0; i < n; ++i) {
+        const int64_t one = int64_t(1) << 30;
+        if (rope_cos[i] < -one || rope_cos[i] > one || rope_sin[i] < -one || rope_sin[i] > one)
+            return fail(EII_ERR_ARG, "rope table entry %zu lies outside [-2^30, 2^30]", i);
+        h[PAGED_DMAX + 1 + i] = static_cast<int32_t>(rope_cos[i]);
+        h[PAGED_DMAX + 1 + n + i] = static_cast<int32_t>(rope_sin[i]);
+    }
+    TRY(check_device(device));
+    DeviceGuard dg(device);
+    CK(dg.st);
+    eii_paged* p = new (std::nothrow) eii_paged;
+    if (!p) return fail(EII_ERR_ARG, "out of host memory");
+    p->device = device;
+    p->n_heads = n_heads; p->n_kv = n_kv; p->hd = head_dim; p->bits = cache_bits; p->n_pos = n_pos;
+    while ((1 << p->page_shift) < page_size) ++p->page_shift;
+    const size_t exp_bytes = (PAGED_DMAX + 1 + 3) / 4 * 16, rope_bytes = n * 4;  // rope rows stay 16-byte aligned
+    int rc = EII_OK;
+    if (cudaDeviceGetAttribute(&p->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaMalloc(&p->mem, exp_bytes + 2 * rope_bytes + 16) != cudaSuccess)
+        rc = fail(EII_ERR_CUDA, "device memory for the cache's tables: %s", cudaGetErrorString(cudaGetLastError()));
+    if (rc == EII_OK) {
+        p->exp_tab = reinterpret_cast<int32_t*>(p->mem);
+        p->rope_c = reinterpret_cast<int32_t*>(p->mem + exp_bytes);
+        p->rope_s = reinterpret_cast<int32_t*>(p->mem + exp_bytes + rope_bytes);
+        p->err = reinterpret_cast<int*>(p->mem + exp_bytes + 2 * rope_bytes);
+        if (cudaMemcpy(p->exp_tab, h.data(), (PAGED_DMAX + 1) * 4, cudaMemcpyHostToDevice) != cudaSuccess ||
+            cudaMemcpy(p->rope_c, h.data() + PAGED_DMAX + 1, 2 * rope_bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
+            cudaMemset(p->err, 0, sizeof(int)) != cudaSuccess)
+            rc = fail(EII_ERR_CUDA, "table upload failed: %s", cudaGetErrorString(cudaGetLastError()));
+    }
+    if (rc != EII_OK) {
+        cudaFree(p->mem);
+        delete p;
+        return rc;
+    }
+    *out = p;
+    return EII_OK;
+}
+
+int64_t eii_paged_pool_bytes(const eii_paged* p, int64_t n_pages) {
+    if (!p) return -static_cast<int64_t>(fail(EII_ERR_ARG, "cache is null"));
+    if (n_pages < 1 || n_pages > INT32_MAX)
+        return -static_cast<int64_t>(fail(EII_ERR_ARG, "n_pages must be in [1, 2^31) (got %lld)", (long long)n_pages));
+    return n_pages * p->n_kv * slab_bytes(p);
+}
+
+int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                     const void* v, int64_t ldv, int in_bits, int n_rows, const int32_t* seq, const int32_t* pos,
+                     int shift_q, int shift_k, int16_t* q_out, int64_t ldqo, int32_t* kv_out, void* stream) {
+    if (!p) return fail(EII_ERR_ARG, "cache is null");
+    TRY(check_pages(p, pages));
+    if (!k || !v || !pos) return fail(EII_ERR_ARG, "k, v or pos is null");
+    if (!q != !q_out) return fail(EII_ERR_ARG, "q and q_out come together");
+    if (in_bits != 16 && in_bits != 32) return fail(EII_ERR_ARG, "in_bits must be 16 or 32 (got %d)", in_bits);
+    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (!seq && n_rows > pages->n_seq)
+        return fail(EII_ERR_ARG, "%d rows without sequence indices but %d sequences", n_rows, pages->n_seq);
+    TRY(check_ld("ldk", ldk, (int64_t)p->n_kv * p->hd));
+    TRY(check_ld("ldv", ldv, (int64_t)p->n_kv * p->hd));
+    if (q) {
+        TRY(check_ld("ldq", ldq, (int64_t)p->n_heads * p->hd));
+        TRY(check_ld("ldqo", ldqo, (int64_t)p->n_heads * p->hd));
+        TRY(check_shift("shift_q", shift_q));
+    }
+    TRY(check_shift("shift_k", shift_k));
+    const uintptr_t in = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
+    if (in & (in_bits / 8 - 1)) return fail(EII_ERR_ARG, "q, k and v must be aligned to their elements");
+    if (n_rows == 0) return EII_OK;
+    DeviceGuard dg(p->device);
+    CK(dg.st);
+    AppendParams ap{};
+    ap.g = geometry(p, pages);
+    ap.q = q; ap.k = k; ap.v = v; ap.ldq = ldq; ap.ldk = ldk; ap.ldv = ldv; ap.n_rows = n_rows; ap.seq = seq; ap.pos = pos;
+    ap.rope_c = p->rope_c; ap.rope_s = p->rope_s; ap.n_pos = p->n_pos; ap.shift_q = shift_q; ap.shift_k = shift_k;
+    ap.q_out = q_out; ap.ldqo = ldqo; ap.kv_out = kv_out;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->hd == 64) return p->bits == 4 ? launch_append<64, 4>(ap, in_bits, st) : launch_append<64, 16>(ap, in_bits, st);
+    return p->bits == 4 ? launch_append<128, 4>(ap, in_bits, st) : launch_append<128, 16>(ap, in_bits, st);
+}
+
+int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, int64_t ldq, int n_rows,
+                        const int32_t* seq, const int32_t* len, int max_len, int shift_s, int prob_bits, int shift_c,
+                        int bits_c, int32_t* ctx, int64_t ldc, void* stream) {
+    if (!p) return fail(EII_ERR_ARG, "cache is null");
+    TRY(check_pages(p, pages));
+    if (!q || !len || !ctx) return fail(EII_ERR_ARG, "q, len or ctx is null");
+    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (!seq && n_rows > pages->n_seq)
+        return fail(EII_ERR_ARG, "%d rows without sequence indices but %d sequences", n_rows, pages->n_seq);
+    if (max_len < 0 || max_len > EII_PAGED_MAX_LEN)
+        return fail(EII_ERR_ARG, "max_len must be in [0, %d] (got %d)", EII_PAGED_MAX_LEN, max_len);
+    TRY(check_ld("ldq", ldq, (int64_t)p->n_heads * p->hd));
+    TRY(check_ld("ldc", ldc, (int64_t)p->n_heads * p->hd));
+    TRY(check_shift("shift_s", shift_s));
+    TRY(check_shift("shift_c", shift_c));
+    if (prob_bits < 16 || prob_bits > 19) return fail(EII_ERR_ARG, "prob_bits must be in [16, 19] (got %d)", prob_bits);
+    if (bits_c < 2 || bits_c > 32) return fail(EII_ERR_ARG, "bits_c must be in [2, 32] (got %d)", bits_c);
+    if ((reinterpret_cast<uintptr_t>(q) & 1) || (reinterpret_cast<uintptr_t>(ctx) & 3))
+        return fail(EII_ERR_ARG, "q and ctx must be aligned to their elements");
+    if (n_rows == 0) return EII_OK;
+    DeviceGuard dg(p->device);
+    CK(dg.st);
+    PagedAttnParams ap{};
+    ap.g = geometry(p, pages);
+    ap.q = q; ap.ldq = ldq; ap.n_rows = n_rows; ap.seq = seq; ap.len = len; ap.max_len = max_len;
+    ap.shift_s = shift_s; ap.prob_bits = prob_bits; ap.shift_c = shift_c; ap.bits_c = bits_c; ap.ctx = ctx; ap.ldc = ldc;
+    const int64_t blocks = (int64_t)n_rows * p->n_heads;
+    if (blocks > INT32_MAX) return fail(EII_ERR_ARG, "n_rows %d is too large", n_rows);
+    k_paged_attention<<<(unsigned)blocks, 128, 0, static_cast<cudaStream_t>(stream)>>>(ap);
+    CK(cudaGetLastError());
+    return EII_OK;
+}
+
+int eii_paged_sync(eii_paged* p, void* stream) {
+    if (!p) return fail(EII_ERR_ARG, "cache is null");
+    DeviceGuard dg(p->device);
+    CK(dg.st);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int code = 0;
+    CK(cudaMemcpyAsync(&code, p->err, sizeof(int), cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    if (!code) return EII_OK;
+    CK(cudaMemsetAsync(p->err, 0, sizeof(int), st));
+    CK(cudaStreamSynchronize(st));
+    switch (code) {
+        case ERR_PAGED_SEQ: return fail(EII_ERR_ARG, "a row's sequence index is not below n_seq");
+        case ERR_PAGED_POS: return fail(EII_ERR_ARG, "a row's position lies outside the rope table or the page table");
+        case ERR_PAGED_PAGE: return fail(EII_ERR_ARG, "the page table names a page outside [0, n_pages)");
+        case ERR_PAGED_LEN: return fail(EII_ERR_ARG, "a row's length exceeds max_len or the page table");
+        case ERR_PAGED_INPUT: return fail(EII_ERR_ARG, "a q, k or v value lies outside the int16 range");
+    }
+    return fail(EII_ERR_DEVICE, "kernel reported error %d", code);
+}
+
+void eii_paged_close(eii_paged* p) {
+    if (!p) return;
+    DeviceGuard dg(p->device);
+    cudaFree(p->mem);
+    delete p;
+}
+
+}  // extern "C"

@@ -1,0 +1,84 @@
+// C ABI of eii_sample: argument checks, handle, launch.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <new>
+
+#include "eii.h"
+#include "eii_host.h"
+#include "eii_sample.cuh"
+
+using namespace eii;
+
+struct eii_sampler {
+    int device = 0, num_sms = 0;
+    int* err = nullptr;
+};
+
+extern "C" {
+
+int eii_sampler_open(int device, eii_sampler** out) {
+    if (!out) return fail(EII_ERR_ARG, "out is null");
+    *out = nullptr;
+    TRY(check_device(device));
+    DeviceGuard dg(device);
+    CK(dg.st);
+    eii_sampler* s = new (std::nothrow) eii_sampler;
+    if (!s) return fail(EII_ERR_ARG, "out of host memory");
+    s->device = device;
+    if (cudaDeviceGetAttribute(&s->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaMalloc(&s->err, 16) != cudaSuccess || cudaMemset(s->err, 0, 16) != cudaSuccess) {
+        const int rc = fail(EII_ERR_CUDA, "sampler set-up failed: %s", cudaGetErrorString(cudaGetLastError()));
+        cudaFree(s->err);
+        delete s;
+        return rc;
+    }
+    *out = s;
+    return EII_OK;
+}
+
+int eii_sample(eii_sampler* s, const int32_t* logits, int64_t ld, int n_rows, int vocab, const int32_t* inv_temp,
+               const int32_t* top_k, const int32_t* top_p, const int32_t* min_p, const uint32_t* u, int64_t* token,
+               int32_t* kept, int32_t* prob, void* stream) {
+    if (!s) return fail(EII_ERR_ARG, "sampler is null");
+    if (!logits || !u || !token) return fail(EII_ERR_ARG, "logits, u or token is null");
+    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return fail(EII_ERR_ARG, "vocab must be in [1, %d] (got %d)", SAMPLE_MAX_VOCAB, vocab);
+    if (ld < vocab) return fail(EII_ERR_ARG, "ld must be >= %d (got %lld)", vocab, (long long)ld);
+    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(u)) & 3)
+        return fail(EII_ERR_ARG, "logits and u must be 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(token) & 7) return fail(EII_ERR_ARG, "token must be 8-byte aligned");
+    if (n_rows == 0) return EII_OK;
+    DeviceGuard dg(s->device);
+    CK(dg.st);
+    SampleParams p{};
+    p.logits = logits; p.ld = ld; p.n_rows = n_rows; p.vocab = vocab; p.inv_temp = inv_temp; p.top_k = top_k;
+    p.top_p = top_p; p.min_p = min_p; p.u = u; p.token = token; p.kept = kept; p.prob = prob; p.err = s->err;
+    k_sample<<<n_rows, SAMPLE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    CK(cudaGetLastError());
+    return EII_OK;
+}
+
+int eii_sampler_sync(eii_sampler* s, void* stream) {
+    if (!s) return fail(EII_ERR_ARG, "sampler is null");
+    DeviceGuard dg(s->device);
+    CK(dg.st);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int code = 0;
+    CK(cudaMemcpyAsync(&code, s->err, sizeof(int), cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    if (!code) return EII_OK;
+    CK(cudaMemsetAsync(s->err, 0, sizeof(int), st));
+    CK(cudaStreamSynchronize(st));
+    if (code == ERR_SAMPLE_PARAM) return fail(EII_ERR_ARG, "a row's sampling parameter lies outside its range");
+    return fail(EII_ERR_DEVICE, "kernel reported error %d", code);
+}
+
+void eii_sampler_close(eii_sampler* s) {
+    if (!s) return;
+    DeviceGuard dg(s->device);
+    cudaFree(s->err);
+    delete s;
+}
+
+}  // extern "C"

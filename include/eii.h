@@ -222,6 +222,92 @@ int eii_linear_noalloc(const int64_t* a_dev, int M, int K, int bits_in, const in
                        const int64_t* n_dev, int N, int f_in, int f_out, int bits_out, int64_t* out_dev,
                        int64_t* acc_dev, void* stream);
 
+/* Paged K/V cache for ragged batches (no reference counterpart): rows of different sequences, each at
+ * a position of its own, appended to and attended over in pages that the caller hands out.  The cache
+ * is kept at 16 bits -- the integers of the engine's own decoder -- or compressed to 4.  Device
+ * pointers throughout; the pools, the page table and all outputs belong to the caller.  The calls
+ * enqueue on `stream` (a cudaStream_t, null = the legacy default stream) and return; they allocate
+ * nothing, keep nothing between calls and can be captured into a CUDA graph.  Calls of one handle may
+ * run at the same time on several streams as long as their outputs do not overlap.  The caller's
+ * current device is left as it was.  Argument errors are returned at once; device-side errors (an
+ * index outside its range) are kept in the handle until the next eii_paged_sync, and the row concerned
+ * is skipped or, with a page index out of range, has an undefined context row.
+ *
+ * A pool is [n_pages][n_kv] slabs of page_size positions.  16 bits: int16 [page_size][head_dim].
+ * 4 bits: uint8 [page_size][head_dim / 2], then uint32 [page_size][head_dim / 64]; each group of 64
+ * dimensions has a scale word m | (z & 0xffff) << 16 and 32 bytes, byte j with dimension j in the low
+ * and j + 32 in the high nibble; nibble n stands for z + m n with z = min, m = max(1, ceil((max -
+ * min) / 15)), n = floor((2 (x - z) + m) / (2 m)) over the group.
+ *
+ * eii_paged_open: head_dim 64 or 128, page_size a power of two in [16, 1024], cache_bits 4 or 16,
+ * n_heads a multiple of n_kv (query head h reads kv head h / (n_heads / n_kv)).  rope_cos, rope_sin:
+ * host Q30 tables [n_pos][head_dim / 2], |entry| <= 2^30, copied; both null = the tables of
+ * eii_table_rope (head_dim 64).
+ * eii_paged_pool_bytes: bytes of one of the two pools, or minus an error code. */
+#define EII_PAGED_MAX_LEN 131072
+typedef struct eii_paged eii_paged;
+/* The pools (16-byte aligned) and page table of one layer: position t of sequence s lies in page
+ * table[s * ld_table + t / page_size].  Entries that a call does not reach may hold anything. */
+typedef struct eii_pages {
+    void *k_pool, *v_pool;
+    int64_t n_pages;
+    const int32_t* table; /* [n_seq][ld_table] */
+    int64_t ld_table;
+    int n_seq;
+} eii_pages;
+int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_size, int cache_bits, int n_pos,
+                   const int64_t* rope_cos, const int64_t* rope_sin, eii_paged** out);
+int64_t eii_paged_pool_bytes(const eii_paged* p, int64_t n_pages);
+/* Appends n_rows rows: row r belongs to sequence seq[r] (null: r) at position pos[r]; with either
+ * negative it is padding, and its outputs are left as they were.  k, v (and q, nullable) hold in_bits
+ * 16 or 32 integers within int16, rows ldk / ldv / ldq elements apart.  q and k are rotated as
+ * python/intref.py:212-225,
+ *   o[d] = SAT16(RS(a[d] cos - a[d + hd/2] sin, shift)), o[d + hd/2] = SAT16(RS(a[d + hd/2] cos + a[d] sin, shift)),
+ * with shift = 30 + f_in - f_out in [1, 62]; the rotated q rows go to q_out int16 (ldqo apart; may be
+ * q itself when in_bits is 16 and ldqo = ldq), the rotated k and the v rows to the cache.  kv_out
+ * (nullable) int32 [n_rows][2][n_kv][head_dim] receives the k and v values that the cache now stands
+ * for.  The rows of one call have distinct places in the pools. */
+int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                     const void* v, int64_t ldv, int in_bits, int n_rows, const int32_t* seq, const int32_t* pos,
+                     int shift_q, int shift_k, int16_t* q_out, int64_t ldqo, int32_t* kv_out, void* stream);
+/* Attention of n_rows query rows: row r (rotated q, int16) sees positions 0 .. len[r] - 1 of sequence
+ * seq[r] (null: r; negative: the row is left as it was; a sequence may have several rows, each with
+ * its own length).  Per query head, with values as the cache holds them (python/intref.py:227-254):
+ *   s_j = SAT16(RS(q . k_j, shift_s)), e_j = E[max s - s_j] (0 beyond 1536), Z = sum e_j,
+ *   P_j = floor((e_j 2^prob_bits + floor(Z / 2)) / Z),  ctx = SAT(RS(sum_j P_j v_j, shift_c), bits_c)
+ * to ctx int32 rows of ldc elements.  prob_bits 16 gives the engine's attention; up to 19 keeps small
+ * probabilities of long sequences.  shift_c = prob_bits + f_v - f_ctx.  len[r] <= 0 gives zeros;
+ * len[r] <= max_len <= EII_PAGED_MAX_LEN. */
+int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, int64_t ldq, int n_rows,
+                        const int32_t* seq, const int32_t* len, int max_len, int shift_s, int prob_bits, int shift_c,
+                        int bits_c, int32_t* ctx, int64_t ldc, void* stream);
+/* Waits for `stream` and reports (and clears) a device-side error of the handle's calls. */
+int eii_paged_sync(eii_paged* p, void* stream);
+/* The caller closes the handle after its last call has finished. */
+void eii_paged_close(eii_paged* p);
+
+/* Drawing the next tokens from integer logits and given random words, all in integers (no reference
+ * counterpart).  Row r of logits (int32, exponent 16 as eii_forward writes them, ld elements apart,
+ * INT32_MIN = a token that must not be drawn) with M its maximum has weights
+ *   w_v ~ 2^30 exp(-(M - l_v) / T), integer, 0 below 2^-31 of the maximum's,
+ * defined in csrc/eii_sample.cuh.  In the order weight descending, index ascending, the first top_k
+ * tokens are kept; of these those with w >= min_p w_max; of these the shortest prefix whose mass
+ * reaches top_p of their mass (at least one).  The token is the lowest index at which the running
+ * kept mass, in index order, exceeds floor(u mass / 2^32).  A row of masked logits only gives -1.
+ * Per-row parameters on the device, null = off: inv_temp 1/T in Q16, [1, 2^22] (null: T = 1), top_k
+ * >= 0 (0: off), top_p and min_p in Q16, [0, 65536] (65536 / 0: off).  top_k = 1 is the greedy choice.
+ * u uint32 [n_rows].  Outputs: token int64 [n_rows]; nullable kept int32 (tokens kept) and prob int32
+ * (Q30 probability of the token among the kept, rounded to nearest).  vocab in [1, 262144].
+ * A parameter outside its range gives -1 and an error at eii_sampler_sync.  Enqueues on `stream`
+ * (null = the legacy default stream) and returns; allocates nothing and can be captured. */
+typedef struct eii_sampler eii_sampler;
+int eii_sampler_open(int device, eii_sampler** out);
+int eii_sample(eii_sampler* s, const int32_t* logits, int64_t ld, int n_rows, int vocab, const int32_t* inv_temp,
+               const int32_t* top_k, const int32_t* top_p, const int32_t* min_p, const uint32_t* u, int64_t* token,
+               int32_t* kept, int32_t* prob, void* stream);
+int eii_sampler_sync(eii_sampler* s, void* stream);
+void eii_sampler_close(eii_sampler* s);
+
 /* Per-kernel timing.  While enabled, every launch of the engine is bracketed by CUDA events on
  * its stream (this adds a few microseconds per launch, so time whole runs with it off).
  * eii_profile_enable resets the counters; eii_profile_read returns the summed device time (ms)
