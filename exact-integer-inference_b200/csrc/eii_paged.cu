@@ -69,6 +69,38 @@ int launch_append(const AppendParams& ap, int in_bits, cudaStream_t st) {
     return EII_OK;
 }
 
+// Launch shape of the attention.  Warps per block: eight, or as few as the longest sequence has tiles.
+// Blocks per cluster: the power of two that gives the GPU about 16 warps per SM, as long as every warp
+// has a tile, and at least as many as the scores need.
+template <int HD, int BITS>
+int launch_attention(const eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
+    using C = PattnCfg<HD, BITS>;
+    const int tiles = (ap.max_len + 31) / 32;
+    const int64_t items = static_cast<int64_t>(ap.n_rows) * p->n_kv * ((ap.g.group + PATTN_HEADS - 1) / PATTN_HEADS);
+    const int warps = tiles >= 8 ? 8 : tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
+    int cs = 1;
+    while (cs < PATTN_MAX_CLUSTER && ((tiles + cs - 1) / cs * 32 > PATTN_MAX_PART ||
+                                      (items * cs * warps < 16 * p->num_sms && 2 * cs * warps <= tiles)))
+        cs *= 2;
+    if (items * cs > INT32_MAX) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
+    const int part = ((tiles + cs - 1) / cs + (tiles == 0)) * 32, smem = C::smem(warps, part);
+    CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (cs > 8) CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(items * cs));
+    cfg.blockDim = dim3(32 * warps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cs;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = cs > 1 ? 1 : 0;
+    CK(cudaLaunchKernelEx(&cfg, k_paged_attention<HD, BITS>, ap, cs, part));
+    return EII_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -212,11 +244,9 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
     ap.g = geometry(p, pages);
     ap.q = q; ap.ldq = ldq; ap.n_rows = n_rows; ap.seq = seq; ap.len = len; ap.max_len = max_len;
     ap.shift_s = shift_s; ap.prob_bits = prob_bits; ap.shift_c = shift_c; ap.bits_c = bits_c; ap.ctx = ctx; ap.ldc = ldc;
-    const int64_t blocks = (int64_t)n_rows * p->n_heads;
-    if (blocks > INT32_MAX) return fail(EII_ERR_ARG, "n_rows %d is too large", n_rows);
-    k_paged_attention<<<(unsigned)blocks, 128, 0, static_cast<cudaStream_t>(stream)>>>(ap);
-    CK(cudaGetLastError());
-    return EII_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->hd == 64) return p->bits == 4 ? launch_attention<64, 4>(p, ap, st) : launch_attention<64, 16>(p, ap, st);
+    return p->bits == 4 ? launch_attention<128, 4>(p, ap, st) : launch_attention<128, 16>(p, ap, st);
 }
 
 int eii_paged_sync(eii_paged* p, void* stream) {
