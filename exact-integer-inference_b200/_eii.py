@@ -406,6 +406,10 @@ class Pages(ctypes.Structure):
     _fields_ = [("k_pool", _P), ("v_pool", _P), ("n_pages", ctypes.c_int64), ("table", _P), ("ld_table", ctypes.c_int64),
                 ("n_seq", ctypes.c_int)]
 
+    @property
+    def ref(self):
+        return ctypes.addressof(self)
+
 
 class Paged:
     """Paged K/V cache of 16 or 4 bits (include/eii.h, eii_paged_*).  Pointers are device pointers on
@@ -448,16 +452,20 @@ class Paged:
 
     def append(self, pages, k_ptr, v_ptr, n_rows, pos_ptr, shift_k, seq_ptr=None, q_ptr=None, q_out_ptr=None, shift_q=1,
                in_bits=16, ldq=None, ldk=None, ldv=None, ldqo=None, kv_out_ptr=None, stream=None):
-        check(lib().eii_paged_append(self.h, ctypes.byref(pages), q_ptr, self.q_row if ldq is None else ldq, k_ptr,
-                                     self.kv_row if ldk is None else ldk, v_ptr, self.kv_row if ldv is None else ldv,
-                                     int(in_bits), int(n_rows), seq_ptr, pos_ptr, int(shift_q), int(shift_k), q_out_ptr,
-                                     self.q_row if ldqo is None else ldqo, kv_out_ptr, stream))
+        rc = _lib.eii_paged_append(self.h, pages.ref, q_ptr, self.q_row if ldq is None else ldq, k_ptr,
+                                   self.kv_row if ldk is None else ldk, v_ptr, self.kv_row if ldv is None else ldv, in_bits,
+                                   n_rows, seq_ptr, pos_ptr, shift_q, shift_k, q_out_ptr,
+                                   self.q_row if ldqo is None else ldqo, kv_out_ptr, stream)
+        if rc:
+            check(rc)
 
     def attention(self, pages, q_ptr, n_rows, len_ptr, max_len, shift_s, shift_c, bits_c, out_ptr, seq_ptr=None,
                   prob_bits=16, ldq=None, ldc=None, stream=None):
-        check(lib().eii_paged_attention(self.h, ctypes.byref(pages), q_ptr, self.q_row if ldq is None else ldq,
-                                        int(n_rows), seq_ptr, len_ptr, int(max_len), int(shift_s), int(prob_bits),
-                                        int(shift_c), int(bits_c), out_ptr, self.q_row if ldc is None else ldc, stream))
+        rc = _lib.eii_paged_attention(self.h, pages.ref, q_ptr, self.q_row if ldq is None else ldq, n_rows, seq_ptr, len_ptr,
+                                      max_len, shift_s, prob_bits, shift_c, bits_c, out_ptr,
+                                      self.q_row if ldc is None else ldc, stream)
+        if rc:
+            check(rc)
 
     def sync(self, stream=None):
         check(lib().eii_paged_sync(self.h, stream))
@@ -486,8 +494,10 @@ class Sampler:
 
     def sample(self, logits_ptr, n_rows, vocab, u_ptr, token_ptr, ld=None, inv_temp_ptr=None, top_k_ptr=None,
                top_p_ptr=None, min_p_ptr=None, kept_ptr=None, prob_ptr=None, stream=None):
-        check(lib().eii_sample(self.h, logits_ptr, vocab if ld is None else ld, int(n_rows), int(vocab), inv_temp_ptr,
-                               top_k_ptr, top_p_ptr, min_p_ptr, u_ptr, token_ptr, kept_ptr, prob_ptr, stream))
+        rc = _lib.eii_sample(self.h, logits_ptr, vocab if ld is None else ld, n_rows, vocab, inv_temp_ptr, top_k_ptr,
+                             top_p_ptr, min_p_ptr, u_ptr, token_ptr, kept_ptr, prob_ptr, stream)
+        if rc:
+            check(rc)
 
     def sync(self, stream=None):
         check(lib().eii_sampler_sync(self.h, stream))

@@ -69,36 +69,95 @@ int launch_append(const AppendParams& ap, int in_bits, cudaStream_t st) {
     return EII_OK;
 }
 
-// Launch shape of the attention.  Warps per block: eight, or as few as the longest sequence has tiles.
-// Blocks per cluster: the power of two that gives the GPU about 16 warps per SM, as long as every warp
-// has a tile, and at least as many as the scores need.
-template <int HD, int BITS>
-int launch_attention(const eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
-    using C = PattnCfg<HD, BITS>;
-    const int tiles = (ap.max_len + 31) / 32;
-    const int64_t items = static_cast<int64_t>(ap.n_rows) * p->n_kv * ((ap.g.group + PATTN_HEADS - 1) / PATTN_HEADS);
-    const int warps = tiles >= 8 ? 8 : tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
-    int cs = 1;
-    while (cs < PATTN_MAX_CLUSTER && ((tiles + cs - 1) / cs * 32 > PATTN_MAX_PART ||
-                                      (items * cs * warps < 16 * p->num_sms && 2 * cs * warps <= tiles)))
+constexpr int kSmemOptin = 227 * 1024 - 3072;  // dynamic shared memory of one block beside the static words
+
+// How the work of one attention call is laid out.
+struct AttnShape {
+    bool warp;      // one warp per item
+    int warps, cs;  // warps per block, blocks per cluster
+};
+
+// Measured in captured graphs (9 query heads on 3 kv heads, head_dim 64, 4 bits unless said, us):
+//  - one warp per item once items fill the SMs and none is long: 4096 x 128 keys 56 (two warps per item 90,
+//    eight 193), at 16 bits 94 (140); 512 x 512 at 16 bits 50 (four warps 60); but 64 x 512 10.2 with eight.
+//    A warp's fixed cost is about two tiles' work.
+//  - eight warps otherwise: 64 x 512 10.2 (four 11.8); four when there are many items of at most 1024 keys.
+//  - clusters until there are eight warps per SM and as long as a warp keeps two tiles: 8 x 4096 13.7 with
+//    eight blocks (four 14.0, sixteen 25.5), 1 x 4096 11.1 (sixteen 11.7), 8 x 32768 42.6 (sixteen 53.6);
+//    two blocks more for long sequences that would leave a tail (64 x 4096 32.4, one block over 39) or whose
+//    scores (nh int16 per key) would keep a second block off the SM: 128 rows x 6000 keys of 32 heads on 8 of
+//    head_dim 128 276 with two blocks, 370 with one.
+//  - sixteen warps for the longest of a few sequences: 1 x 65521 30 (eight 36).
+AttnShape attn_shape(int64_t items, int tiles, int nh, int sms) {
+    if (tiles <= 32 && items >= 8 * sms) return {true, 4, 1};
+    int warps = 1, cs = 1;
+    while (warps < 8 && warps < tiles) warps *= 2;
+    if (warps == 8 && tiles <= 32 && items >= 4 * sms) warps = 4;
+    while (cs < PATTN_MAX_CLUSTER &&
+           ((tiles + cs - 1) / cs * 32 > PATTN_MAX_PART || (items * cs * warps < 8 * sms && 4 * cs * warps <= tiles) ||
+            (cs < 4 && items * cs * warps < 16 * sms && 16 * cs * warps <= tiles) || (cs < 4 && nh * ((tiles + cs - 1) / cs) > 600)))
         cs *= 2;
-    if (items * cs > INT32_MAX) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
-    const int part = ((tiles + cs - 1) / cs + (tiles == 0)) * 32, smem = C::smem(warps, part);
-    CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (cs > 8) CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (cs == PATTN_MAX_CLUSTER && items * cs * 16 <= 8 * sms && 4 * cs * warps <= tiles) warps = 16;
+    return {false, warps, cs};
+}
+
+template <int HD, int BITS, int NH>
+int launch_attention_nh(const eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
+    using C = PattnCfg<HD, BITS, NH>;
+    const int tiles = (ap.max_len + 31) / 32 + (ap.max_len == 0);
+    const int64_t items = static_cast<int64_t>(ap.n_rows) * p->n_kv * ((ap.g.group + NH - 1) / NH);
+    if (items > INT32_MAX / PATTN_MAX_CLUSTER) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
+    AttnShape s = attn_shape(items, tiles, NH, p->num_sms);
+    if (s.warp) {
+        k_paged_attention<HD, BITS, NH, true><<<static_cast<unsigned>((items + s.warps - 1) / s.warps), 32 * s.warps,
+                                               C::smem_warp(s.warps, tiles * 32), st>>>(ap, 1, tiles * 32, static_cast<int>(items));
+        CK(cudaGetLastError());
+        return EII_OK;
+    }
+    const int part = (tiles + s.cs - 1) / s.cs * 32;
+    if (C::smem_block(s.warps, part) > kSmemOptin) s.warps = 8;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(items * cs));
-    cfg.blockDim = dim3(32 * warps);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
+    cfg.blockDim = dim3(32 * s.warps);
+    cfg.gridDim = dim3(static_cast<unsigned>(items * s.cs));
+    cfg.dynamicSmemBytes = C::smem_block(s.warps, part);
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = cs;
+    at.val.clusterDim.x = s.cs;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
-    cfg.numAttrs = cs > 1 ? 1 : 0;
-    CK(cudaLaunchKernelEx(&cfg, k_paged_attention<HD, BITS>, ap, cs, part));
+    cfg.numAttrs = s.cs > 1 ? 1 : 0;
+    CK(cudaLaunchKernelEx(&cfg, k_paged_attention<HD, BITS, NH, false>, ap, s.cs, part, static_cast<int>(items)));
     return EII_OK;
+}
+
+template <int HD, int BITS>
+int launch_attention(const eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
+    switch (ap.g.group) {
+        case 1: return launch_attention_nh<HD, BITS, 1>(p, ap, st);
+        case 2: return launch_attention_nh<HD, BITS, 2>(p, ap, st);
+        case 3: return launch_attention_nh<HD, BITS, 3>(p, ap, st);
+    }
+    return launch_attention_nh<HD, BITS, 4>(p, ap, st);
+}
+
+// Once per handle: the attention kernels' shared memory and cluster limits on the current device.
+template <int HD, int BITS, int NH>
+int allow_attention() {
+    static_assert(PattnCfg<HD, BITS, NH>::smem_block(8, PATTN_MAX_PART) <= kSmemOptin && PattnCfg<HD, BITS, NH>::smem_warp(4, 1024) <= kSmemOptin, "shared memory");
+    CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptin));
+    CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOptin));
+    CK(cudaFuncSetAttribute(k_paged_attention<HD, BITS, NH, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    return EII_OK;
+}
+template <int HD, int BITS>
+int allow_attention(int group) {
+    switch (group) {
+        case 1: return allow_attention<HD, BITS, 1>();
+        case 2: return allow_attention<HD, BITS, 2>();
+        case 3: return allow_attention<HD, BITS, 3>();
+    }
+    return allow_attention<HD, BITS, 4>();
 }
 
 }  // namespace
@@ -168,6 +227,9 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
             cudaMemset(p->err, 0, sizeof(int)) != cudaSuccess)
             rc = fail(EII_ERR_CUDA, "table upload failed: %s", cudaGetErrorString(cudaGetLastError()));
     }
+    const int group = n_heads / n_kv;
+    if (rc == EII_OK && head_dim == 64) rc = cache_bits == 4 ? allow_attention<64, 4>(group) : allow_attention<64, 16>(group);
+    else if (rc == EII_OK) rc = cache_bits == 4 ? allow_attention<128, 4>(group) : allow_attention<128, 16>(group);
     if (rc != EII_OK) {
         cudaFree(p->mem);
         delete p;
@@ -188,11 +250,12 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
                      const void* v, int64_t ldv, int in_bits, int n_rows, const int32_t* seq, const int32_t* pos,
                      int shift_q, int shift_k, int16_t* q_out, int64_t ldqo, int32_t* kv_out, void* stream) {
     if (!p) return fail(EII_ERR_ARG, "cache is null");
+    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (n_rows == 0) return EII_OK;
     TRY(check_pages(p, pages));
     if (!k || !v || !pos) return fail(EII_ERR_ARG, "k, v or pos is null");
     if (!q != !q_out) return fail(EII_ERR_ARG, "q and q_out come together");
     if (in_bits != 16 && in_bits != 32) return fail(EII_ERR_ARG, "in_bits must be 16 or 32 (got %d)", in_bits);
-    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
     if (!seq && n_rows > pages->n_seq)
         return fail(EII_ERR_ARG, "%d rows without sequence indices but %d sequences", n_rows, pages->n_seq);
     TRY(check_ld("ldk", ldk, (int64_t)p->n_kv * p->hd));
@@ -205,7 +268,6 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
     TRY(check_shift("shift_k", shift_k));
     const uintptr_t in = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
     if (in & (in_bits / 8 - 1)) return fail(EII_ERR_ARG, "q, k and v must be aligned to their elements");
-    if (n_rows == 0) return EII_OK;
     DeviceGuard dg(p->device);
     CK(dg.st);
     AppendParams ap{};
@@ -222,9 +284,10 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
                         const int32_t* seq, const int32_t* len, int max_len, int shift_s, int prob_bits, int shift_c,
                         int bits_c, int32_t* ctx, int64_t ldc, void* stream) {
     if (!p) return fail(EII_ERR_ARG, "cache is null");
+    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (n_rows == 0) return EII_OK;
     TRY(check_pages(p, pages));
     if (!q || !len || !ctx) return fail(EII_ERR_ARG, "q, len or ctx is null");
-    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
     if (!seq && n_rows > pages->n_seq)
         return fail(EII_ERR_ARG, "%d rows without sequence indices but %d sequences", n_rows, pages->n_seq);
     if (max_len < 0 || max_len > EII_PAGED_MAX_LEN)
@@ -237,7 +300,6 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
     if (bits_c < 2 || bits_c > 32) return fail(EII_ERR_ARG, "bits_c must be in [2, 32] (got %d)", bits_c);
     if ((reinterpret_cast<uintptr_t>(q) & 1) || (reinterpret_cast<uintptr_t>(ctx) & 3))
         return fail(EII_ERR_ARG, "q and ctx must be aligned to their elements");
-    if (n_rows == 0) return EII_OK;
     DeviceGuard dg(p->device);
     CK(dg.st);
     PagedAttnParams ap{};

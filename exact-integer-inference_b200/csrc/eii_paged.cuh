@@ -169,51 +169,69 @@ struct PagedAttnParams {
     int64_t ldc;
 };
 
-// Geometry of the kernel below.  A tile is 32 keys of one warp; a block holds the scores of one part of
-// the keys for up to four query heads in shared memory.
-constexpr int PATTN_HEADS = 4;          // query heads of one block (they share a kv head)
+// Geometry of the kernel below.  A tile is 32 keys of one warp.
+constexpr int PATTN_MAX_HEADS = 4;      // query heads of one item (they share a kv head)
 constexpr int PATTN_MAX_PART = 8192;    // keys of one block: 64 KB of scores
+constexpr int PATTN_MAX_WARPS = 16;     // of one block
 constexpr int PATTN_MAX_CLUSTER = 16;
-constexpr int PATTN_EXP_BYTES = (PAGED_DMAX + 1 + 3) / 4 * 16;
+constexpr int PATTN_EXP_BYTES = (PAGED_DMAX + 2 + 3) / 4 * 16;  // one entry more: zero
 
-template <int HD, int BITS>
+template <int HD, int BITS, int NH>
 struct PattnCfg {
     static constexpr int A = HD / 64;                        // scale groups of a row
     static constexpr int KS = HD / 32;                       // 32-wide steps of the score product
     static constexpr int SWEEPS = BITS == 4 ? 1 : A;         // passes over V (64 accumulators at most per thread)
     static constexpr int GPS = A / SWEEPS;                   // 64-dim groups per sweep
     static constexpr int NT = BITS == 4 ? 8 * GPS : 16;      // 8-column accumulator tiles
+    static constexpr int RR = NH > 2 ? 2 : 1;                // halves of the 16 product rows in use by the context
+    static constexpr int ROW = BITS == 4 ? HD / 2 : HD * 2;  // bytes of a cached row without its scales
+    static constexpr int TILE = 32 * ROW + (BITS == 4 ? 128 * A : 0);
+    static constexpr int STAGES = BITS == 4 && HD == 64 ? 3 : 2;  // tiles of the warp's ring
     static constexpr int RAW_ROW = BITS == 4 ? 40 : 36;      // padded row of 32 raw scores
-    static constexpr int RAW_BYTES = PATTN_HEADS * RAW_ROW * (BITS == 4 ? 4 * A : 8);
-    static constexpr int PLANE_BYTES = 16 * 32 * (BITS == 4 ? A : 1);
-    static constexpr int WARP_BYTES = RAW_BYTES > PLANE_BYTES ? RAW_BYTES : PLANE_BYTES;  // the two uses do not overlap in time
-    static constexpr int ACC_COLS = BITS == 4 ? 64 * GPS : 128;  // columns of the block's accumulator rows
-    static constexpr int ACC_LD = ACC_COLS + 8;
-    static constexpr int ACC_BYTES = 16 * ACC_LD * 4;
-    static constexpr int CTX_BYTES = PATTN_HEADS * HD * 8;
-    static constexpr int smem(int warps, int part) {
-        return PATTN_EXP_BYTES + ACC_BYTES + CTX_BYTES + warps * WARP_BYTES + PATTN_HEADS * part * 2;
+    static constexpr int RAW_BYTES = (NH + 1) * RAW_ROW * (BITS == 4 ? 4 * A : 8);
+    static constexpr int WGT_BYTES = 2 * RR * 32 * 4 * (BITS == 4 ? A : 1);
+    static constexpr int TEMP_BYTES = RAW_BYTES > WGT_BYTES ? RAW_BYTES : WGT_BYTES;  // never in use at once
+    static constexpr int WARP_BYTES = STAGES * TILE + TEMP_BYTES;
+    static constexpr int ACC_LD = 8 * NT + 8;
+    static constexpr int ACC_BYTES = (8 * RR * ACC_LD + 4) * 4;  // four rows further on, one word further on
+    static constexpr int CTX_BYTES = NH * HD * 8;
+    // A warp on its own puts its accumulators over its ring and scores, unless another sweep needs those:
+    // then behind them.
+    __host__ __device__ static constexpr int warp_bytes(int part) {
+        const int used = WARP_BYTES + NH * part * 2, acc = (ACC_BYTES + 15) / 16 * 16;
+        return SWEEPS > 1 ? used + acc : used > acc ? used : acc;
+    }
+    static constexpr int smem_warp(int warps, int part) { return PATTN_EXP_BYTES + warps * warp_bytes(part); }
+    static constexpr int smem_block(int warps, int part) {
+        return PATTN_EXP_BYTES + ACC_BYTES + CTX_BYTES + warps * WARP_BYTES + NH * part * 2;
     }
 };
 
-// D += A B on 16 x 8 x 32 bytes: A rows are query heads (scores) or head x weight plane (context), B
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// D = A B (+ D) on 16 x 8 x 32 bytes: A rows are query heads (scores) or head x weight byte (context), B
 // columns are keys or dimensions.  A decoding step has a handful of rows, so the 128-row tcgen05 tile
 // would be empty: the warp-level instruction takes its operands from registers, straight from the loads.
-template <bool A_SIGNED, bool B_SIGNED>
-__device__ __forceinline__ void mma_m16n8k32(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    if constexpr (A_SIGNED && B_SIGNED)
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else if constexpr (A_SIGNED)
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else if constexpr (B_SIGNED)
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_s8s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8s8_first(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+__device__ __forceinline__ void mma_u8u8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Byte j of x0..x3 -> r_j (x0's byte lowest).
@@ -226,15 +244,34 @@ __device__ __forceinline__ void transpose4(uint32_t x0, uint32_t x1, uint32_t x2
     r[3] = __byte_perm(t2, t3, 0x7632);
 }
 
-// floor((e 2^pb + floor(z / 2)) / z): the float estimate is off by at most one (e 2^pb / z <= 2^19 with
-// three roundings of 2^-24), which the exact remainder corrects.
-__device__ __forceinline__ uint32_t prob_of(uint32_t e, int pb, uint64_t z, float scale) {
-    const uint64_t num = (static_cast<uint64_t>(e) << pb) + (z >> 1);
-    uint32_t est = static_cast<uint32_t>(__fmaf_rz(static_cast<float>(e), scale, 0.5f));
-    const int64_t rem = static_cast<int64_t>(num - est * z);
-    if (rem < 0) --est;
-    else if (rem >= static_cast<int64_t>(z)) ++est;
-    return est;
+// SAT16(x >> shift) of a score with the rounding half already added.  |x| < 2^38 for every valid cache, so
+// a shift of 8 to 31 leaves 32 bits and one above is taken in two steps; below 8 x is clamped first, which
+// changes only values that saturate.
+struct ScoreShift {
+    int down, rest;
+    bool clamp;
+    int64_t half;
+    __device__ explicit ScoreShift(int shift)
+        : down(min(shift, 32)), rest(max(shift - 32, 0)), clamp(shift < 8), half(int64_t(1) << (shift - 1)) {}
+    __device__ __forceinline__ int32_t operator()(int64_t x) const {
+        if (clamp) x = max(min(x, (int64_t(1) << 30) - 1), -(int64_t(1) << 30));
+        const int32_t s = static_cast<int32_t>(__funnelshift_rc(static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), down)) >> rest;
+        return max(min(s, 32767), -32768);
+    }
+};
+
+// floor((e 2^pb + floor(z / 2)) / z) for e <= 2^30 <= z, with rcp = floor(2^61 / z) <= 2^31: e rcp / 2^(61 - pb)
+// + 1/2 lies above the quotient by at most 1 / (2 z) and below it by less than 2^30 / 2^(61 - pb) <= 2^-12, so
+// its floor is the answer unless its fraction's leading 29 - pb bits are all ones or all zeros
+// (`unsure`, one key in 2^12 at pb = 16); then prob_exact decides by the remainder.
+__device__ __forceinline__ uint32_t prob_of(uint32_t e, int pb, uint32_t rcp, bool& unsure) {
+    const uint32_t hi = static_cast<uint32_t>((static_cast<uint64_t>(e) * rcp + (1ull << (60 - pb))) >> 32);
+    unsure |= ((hi + 1) & ((1u << (29 - pb)) - 1)) <= 1;
+    return hi >> (29 - pb);
+}
+__device__ __forceinline__ uint32_t prob_exact(uint32_t q, uint32_t e, int pb, uint64_t z) {
+    const int64_t rem = static_cast<int64_t>((static_cast<uint64_t>(e) << pb) + (z >> 1) - q * z);
+    return rem < 0 ? q - 1 : rem >= static_cast<int64_t>(z) ? q + 1 : q;
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -260,423 +297,544 @@ __device__ __forceinline__ int64_t ld_remote64(uint32_t a) {
     asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
     return v;
 }
+// Sum of a non-negative v < 2^47 over the warp, in pieces of 24 and 23 bits.
+__device__ __forceinline__ uint64_t warp_sum47(uint64_t v) {
+    const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(v) & 0xFFFFFFu);
+    const uint32_t hi = __reduce_add_sync(~0u, static_cast<uint32_t>(v >> 24));
+    return (static_cast<uint64_t>(hi) << 24) + lo;
+}
+// The same of a signed |v| < 2^50.
+__device__ __forceinline__ int64_t warp_sum_signed(int64_t v) {
+    const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(v) & 0xFFFFFFu);
+    const int32_t hi = __reduce_add_sync(~0u, static_cast<int32_t>(v >> 24));
+    return (static_cast<int64_t>(hi) << 24) + lo;
+}
 
-// One cluster of `cs` blocks per (row, kv head, tile of four query heads); block `rank` takes a contiguous
-// part of the keys, its warps every NW-th tile of 32 of them.  K and V are read once: pass 1 writes
-// SAT16 scores to shared memory and finds the maximum (joined over the cluster), pass 2 sums the
-// exponentials from the scores, pass 3 turns them into probabilities and multiplies V.  All sums are
-// exact integers, so neither the split nor the order changes a result.
-//   scores: q = 256 qh + ql (s8, u8 rows of A); keys are B columns.  4 bits: nibbles are B bytes as they
-//     lie (byte j of a group holds dimensions j and j + 32), s = sum_a m_a (q . n)_a + z_a sum(q_a).
-//     16 bits: k = 256 kh + kl split by byte permutes.
-//   context: 4 bits: W = P m <= 2^19 4369 + 4369 < 2^32 as four u8 planes, sum_j P_j z_j apart; 16 bits:
-//     P as three planes.  Keys run along the product's K: four keys' words are transposed in registers.
-template <int HD, int BITS>
-__global__ void __launch_bounds__(256, BITS == 4 && HD == 64 ? 3 : 2) k_paged_attention(const PagedAttnParams p, const int cs, const int part_cap) {
-    using C = PattnCfg<HD, BITS>;
-    constexpr int H = PATTN_HEADS, A = C::A;
+// An item is (row, kv head, up to NH query heads).  WARP: one warp works on an item by itself (many
+// short sequences).  Otherwise a cluster of `cs` blocks does: block `rank` takes a contiguous part of the
+// keys, its warps every nw-th tile of 32 of them.
+// K and V are read once, as one stream of tiles that each warp copies ahead of itself into a ring in
+// shared memory: pass 1 writes SAT16 scores to shared memory and finds the maximum (joined over the
+// cluster), pass 2 sums the exponentials from the scores, pass 3 turns them into probabilities and
+// multiplies V.  All sums are exact integers, so neither the split nor the order changes a result.
+//   scores: q = 256 qh + 128 + ql with s8 bytes; A holds qh in rows 0..3, ql in rows 8..11 and ones in row
+//     15, keys are B columns, so one product gives qh . k, ql . k and sum(k).  4 bits: nibbles are B bytes as
+//     they lie (byte j of a group holds dimensions j and j + 32), s = sum_a m_a (q . n)_a + z_a sum(q_a).
+//     16 bits: k = 256 kh + 128 + kl split by byte permutes, two products.
+//   context: A holds byte b of head h's weights in row 4 h + b, keys run along the product's K (four keys'
+//     words are transposed in registers), dimensions are columns.  4 bits: W = P m <= 2^19 4369 < 2^32, and
+//     sum_j P_j z_j apart; 16 bits: W = P, the bytes of v in separate columns.
+// An item with fewer heads than NH computes the absent ones from zeros and drops them.
+template <int HD, int BITS, int NH, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512, WARP ? (BITS == 4 && HD == 64 ? 6 : 4) : 1)
+    k_paged_attention(const PagedAttnParams p, const int cs, const int part_cap, const int n_items) {
+    using C = PattnCfg<HD, BITS, NH>;
+    constexpr int A = C::A, S = C::STAGES;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int32_t max_s[H];
-    __shared__ unsigned long long z_s[H];
-    __shared__ uint32_t zlo_s[H * A];  // 8 warps x 32 lanes x 2^24
-    __shared__ int32_t zhi_s[H * A];
+    // each warp's part of a joined value, and (word PATTN_MAX_WARPS) the block's for its cluster; 64-bit shared
+    // atomics are loops and cost 16 warps 7 us
+    constexpr int PARTS = WARP ? 1 : PATTN_MAX_WARPS + 1;
+    __shared__ int32_t max_s[NH][PARTS];
+    __shared__ uint64_t z_s[NH][PARTS];
+    __shared__ int64_t pz_s[NH * A][PARTS];
     const PagedGeom& g = p.g;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
     int32_t* exp_s = reinterpret_cast<int32_t*>(smem);
-    int32_t* acc_s = reinterpret_cast<int32_t*>(smem + PATTN_EXP_BYTES);
-    int64_t* ctx_s = reinterpret_cast<int64_t*>(smem + PATTN_EXP_BYTES + C::ACC_BYTES);
-    uint8_t* stage = smem + PATTN_EXP_BYTES + C::ACC_BYTES + C::CTX_BYTES + warp * C::WARP_BYTES;
-    int16_t* score_s = reinterpret_cast<int16_t*>(smem + PATTN_EXP_BYTES + C::ACC_BYTES + C::CTX_BYTES + nw * C::WARP_BYTES);
+    // block: accumulators, context, ring and temporaries of each warp, scores; warp: ring, temporaries, scores
+    uint8_t* own = smem + PATTN_EXP_BYTES + (WARP ? warp * C::warp_bytes(part_cap) : 0);
+    int32_t* acc_s = reinterpret_cast<int32_t*>(own);
+    int64_t* ctx_s = reinterpret_cast<int64_t*>(own + C::ACC_BYTES);
+    uint8_t* ring = WARP ? own : own + C::ACC_BYTES + C::CTX_BYTES + warp * C::WARP_BYTES;
+    uint8_t* temp = ring + S * C::TILE;
+    int16_t* score_s = reinterpret_cast<int16_t*>(WARP ? own + C::WARP_BYTES
+                                                       : own + C::ACC_BYTES + C::CTX_BYTES + (blockDim.x >> 5) * C::WARP_BYTES);
 
-    const int rank = cs > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int head_tiles = (g.group + H - 1) / H;
-    int item = blockIdx.x / cs;
-    const int ht = item % head_tiles;
-    item /= head_tiles;
-    const int kv = item % g.n_kv, r = item / g.n_kv;
-    const int head0 = kv * g.group + ht * H, nh = min(H, g.group - ht * H);
+    for (int i = tid; i < PATTN_EXP_BYTES / 16; i += blockDim.x) cp_async16(exp_s + 4 * i, g.exp_tab + 4 * i);
+    cp_async_commit();
+    if constexpr (!WARP) {
+        for (int i = tid; i < C::ACC_BYTES / 16; i += blockDim.x) reinterpret_cast<int4*>(acc_s)[i] = make_int4(0, 0, 0, 0);
+    }
+    const int nw = blockDim.x >> 5;
+
+    const int rank = !WARP && cs > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int head_tiles = (g.group + NH - 1) / NH;
+    const int index = WARP ? blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x / cs;
+    const int item = WARP ? min(index, n_items - 1) : index;
+    const int ht = item % head_tiles, kv = item / head_tiles % g.n_kv, r = item / head_tiles / g.n_kv;
+    const int head0 = kv * g.group + ht * NH, nh = min(NH, g.group - ht * NH);
     const int seq = p.seq ? p.seq[r] : r;
-    if (seq < 0) return;  // a padding row (the whole cluster agrees)
-    const int len = max(p.len[r], 0);
-    if (seq >= g.n_seq || len > p.max_len || ((static_cast<int64_t>(len) + (1 << g.page_shift) - 1) >> g.page_shift) > g.ld_table) {
-        if (tid == 0) atomicCAS(g.err, 0, seq >= g.n_seq ? ERR_PAGED_SEQ : ERR_PAGED_LEN);
-        return;
+    int len = max(p.len[r], 0);
+    // a padding row, or one that is refused: all threads of the item agree
+    bool skip = seq < 0 || (WARP && index >= n_items);
+    if (!skip && (seq >= g.n_seq || len > p.max_len ||
+                  ((static_cast<int64_t>(len) + (1 << g.page_shift) - 1) >> g.page_shift) > g.ld_table)) {
+        if (lane == 0) atomicCAS(g.err, 0, seq >= g.n_seq ? ERR_PAGED_SEQ : ERR_PAGED_LEN);
+        skip = true;
     }
+    if (skip) len = 0;
     int32_t* ctx = p.ctx + r * p.ldc + head0 * HD;
-    if (len == 0) {
-        if (rank == 0)
-            for (int i = tid; i < nh * HD; i += blockDim.x) ctx[i] = 0;
-        return;
-    }
+    const int me = WARP ? lane : tid, team = WARP ? 32 : blockDim.x;
     const int32_t* table = g.table + seq * g.ld_table;
     const int tiles = (len + 31) >> 5;
-    const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * rank / cs);
-    const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / cs);
+    const int t0 = WARP ? 0 : static_cast<int>(static_cast<int64_t>(tiles) * rank / cs);
+    const int t1 = WARP ? tiles : static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / cs);
+    const int stride_log2 = WARP ? 0 : 26 - __clz(blockDim.x);  // (a power of two of warps)
+    const int first = WARP ? 0 : t0 + warp;
+    const int n = first < t1 ? ((t1 - 1 - first) >> stride_log2) + 1 : 0;  // this warp's tiles
 
-    for (int i = tid; i <= PAGED_DMAX; i += blockDim.x) exp_s[i] = g.exp_tab[i];
-    for (int i = tid; i < C::ACC_BYTES / 4; i += blockDim.x) acc_s[i] = 0;
-    if (tid < H) {
-        max_s[tid] = -32768;
-        z_s[tid] = 0;
-    }
-    if (tid < H * A) {
-        zlo_s[tid] = 0;
-        zhi_s[tid] = 0;
-    }
-
-    const int gid = lane >> 2, tig = lane & 3;
-    // q fragments: step i of row gid holds dimensions 32 i + 8 tig .. + 7 (two words of each plane)
-    uint32_t qh[C::KS][2], ql[C::KS][2];
-    int32_t qsum[A];
+    // ------------------------------------------------------------ the stream of tiles: K 0..n-1, V 0..n-1 (per sweep)
+    // Lane l holds the page ids of the first (l < 16) or second half of tile number ids_base + (l & 15); pages
+    // hold at least 16 keys, and a half behind the last key repeats the first.
+    const uint32_t page_pitch = static_cast<uint32_t>(g.slab) * g.n_kv;
+    const int slot_mask = (1 << g.page_shift) - 1;
+    int ids = 0, ids_base = 0, tile_i = 0, at_s = 0;  // the next tile to copy and its place in the ring
+    const uint8_t* pool = g.k_pool + kv * g.slab;
+    int sweep_i = -1;                                 // -1: K
+    auto fetch_ids = [&]() {
+        const int i = tile_i + (lane & 15), j = 32 * (first + (i << stride_log2)) + (lane & 16);
+        int x = i < n && j < len ? table[j >> g.page_shift] : 0;
+        const int x0 = __shfl_sync(~0u, x, lane & 15);
+        if (j >= len) x = x0;
+        if (x < 0 || x >= g.n_pages) {
+            atomicCAS(g.err, 0, ERR_PAGED_PAGE);
+            x = 0;
+        }
+        ids = x;
+        ids_base = tile_i;
+    };
+    auto copy_next = [&]() {
+        if (tile_i == n) {
+            tile_i = 0;
+            pool = g.v_pool + kv * g.slab;
+            if (++sweep_i == C::SWEEPS) tile_i = n + 1;  // the stream has ended
+            else if (ids_base != 0) fetch_ids();
+        }
+        if (tile_i < n) {
+            if (tile_i == ids_base + 16) fetch_ids();
+            const int key = 32 * (first + (tile_i << stride_log2));
+            uint8_t* dst = ring + at_s * C::TILE;
+            const uint8_t* half[2];
+            int slot[2];
 #pragma unroll
-    for (int a = 0; a < A; ++a) qsum[a] = 0;
+            for (int h = 0; h < 2; ++h) {
+                slot[h] = (key + 16 * h) & slot_mask;
+                half[h] = pool + static_cast<uint64_t>(static_cast<uint32_t>(__shfl_sync(~0u, ids, tile_i - ids_base + 16 * h))) * page_pitch;
+            }
+            // 16-byte chunks of rows: chunk c of row r lands in chunk c ^ f(r), against bank conflicts
+            constexpr int CH = C::ROW / 16, VCH = BITS == 4 ? CH : CH / C::SWEEPS;
+            if (BITS == 16 && sweep_i >= 0) {
 #pragma unroll
-    for (int i = 0; i < C::KS; ++i) {
+                for (int i = 0; i < VCH; ++i) {
+                    const int row = (lane + 32 * i) / VCH, c = lane % VCH, h = 32 * i >= 16 * VCH;
+                    cp_async16(dst + row * (16 * VCH) + 16 * (c ^ 2 * (row & 3)),
+                               half[h] + (slot[h] + row - 16 * h) * C::ROW + 16 * (c + VCH * sweep_i));
+                }
+            } else {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            uint32_t hi = 0, lo = 0;
-            if (gid < nh) {
-                const int16_t* src = p.q + r * p.ldq + (head0 + gid) * HD + 32 * i + 8 * tig + 4 * w;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int32_t x = src[b];
-                    hi |= (static_cast<uint32_t>(x >> 8) & 0xFFu) << (8 * b);
-                    lo |= (static_cast<uint32_t>(x) & 0xFFu) << (8 * b);
-                    qsum[i >> 1] += x;
+                for (int i = 0; i < CH; ++i) {
+                    const int row = (lane + 32 * i) / CH, c = lane % CH, h = 32 * i >= 16 * CH;
+                    const int f = BITS == 16 ? (row & 1) * 4 : HD == 128 ? (row >> 1 & 1) * 2 : 0;
+                    cp_async16(dst + row * C::ROW + 16 * (c ^ f), half[h] + (slot[h] + row - 16 * h) * C::ROW + 16 * c);
                 }
             }
-            qh[i][w] = hi;
-            ql[i][w] = lo;
-        }
-    }
-    int32_t qs[H][A];  // sum of each head's q over each group, in every lane
-#pragma unroll
-    for (int a = 0; a < A; ++a) {
-        qsum[a] += __shfl_xor_sync(~0u, qsum[a], 1);
-        qsum[a] += __shfl_xor_sync(~0u, qsum[a], 2);
-#pragma unroll
-        for (int h = 0; h < H; ++h) qs[h][a] = __shfl_sync(~0u, qsum[a], 4 * h);
-    }
-
-    // the two pages of a tile (pages hold at least 16 keys); entries behind the last key are not followed
-    auto page_ids = [&](int t, int (&id)[2]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int j = 32 * t + 16 * h;
-            id[h] = j < len ? table[j >> g.page_shift] : -2;
-        }
-    };
-    auto slabs = [&](const uint8_t* pool, const int (&id)[2], int t, const uint8_t* (&s)[2]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int x = id[h] == -2 ? id[0] : id[h];
-            if (x < 0 || x >= g.n_pages) {
-                if (lane == 0) atomicCAS(g.err, 0, ERR_PAGED_PAGE);
-                x = 0;
+            if (BITS == 4 && lane < 8 * A) {
+                const int h = lane >= 4 * A;
+                cp_async16(dst + 32 * C::ROW + 16 * lane,
+                           (h ? half[1] : half[0]) + (C::ROW << g.page_shift) + (h ? slot[1] : slot[0]) * (4 * A) + 16 * (lane - 4 * A * h));
             }
-            s[h] = pool + slab_offset(g, x, kv);
+            ++tile_i;
+            at_s = at_s + 1 == S ? 0 : at_s + 1;
         }
+        cp_async_commit();
     };
-    const int slot_mask = (1 << g.page_shift) - 1;
-    const int scale_at = (HD / 2) << g.page_shift;
+    if (n > 0) fetch_ids();
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+        if (n > 0) copy_next();
+        else cp_async_commit();
+    }
+    cp_async_wait<S - 1>();  // the exp table
+    if (lane < 2 && warp == 0) exp_s[PAGED_DMAX + 1 + lane] = 0;
+    __syncthreads();
+    if (len == 0) {
+        if (!skip && rank == 0)
+            for (int i = me; i < nh * HD; i += team) ctx[i] = 0;
+        return;
+    }
+    int use_s = 0;  // the ring's next tile to use
+    // Waits for that tile, and puts the copy of a later one into the place of the tile used before.
+    auto next_tile = [&]() -> const uint8_t* {
+        cp_async_wait<S - 2>();
+        __syncwarp();
+        copy_next();
+        const uint8_t* x = ring + use_s * C::TILE;
+        use_s = use_s + 1 == S ? 0 : use_s + 1;
+        return x;
+    };
+
+    // q fragments: step i of rows gid and gid + 8 holds dimensions 32 i + 8 tig .. + 7
+    uint32_t qa[C::KS][4];
+    int32_t qc[NH][A];  // sum of a head's q over each group
+    {
+        int32_t v[A];
+#pragma unroll
+        for (int a = 0; a < A; ++a) v[a] = 0;
+        const int16_t* src = p.q + r * p.ldq + (head0 + min(gid, nh - 1)) * HD + 8 * tig;
+        const bool vec = ((reinterpret_cast<uintptr_t>(p.q) | (p.ldq * 2)) & 15) == 0, on = gid < nh;
+#pragma unroll
+        for (int i = 0; i < C::KS; ++i) {
+            uint4 w;
+            if (vec) w = *reinterpret_cast<const uint4*>(src + 32 * i);
+            else {
+                const uint16_t* x = reinterpret_cast<const uint16_t*>(src + 32 * i);
+                w = make_uint4(x[0] | uint32_t(x[1]) << 16, x[2] | uint32_t(x[3]) << 16, x[4] | uint32_t(x[5]) << 16,
+                               x[6] | uint32_t(x[7]) << 16);
+            }
+            const uint32_t none = gid == 7 ? 0x01010101u : 0;
+            qa[i][0] = on ? __byte_perm(w.x, w.y, 0x7531) : 0;
+            qa[i][2] = on ? __byte_perm(w.z, w.w, 0x7531) : 0;
+            qa[i][1] = on ? __byte_perm(w.x, w.y, 0x6420) ^ 0x80808080u : none;
+            qa[i][3] = on ? __byte_perm(w.z, w.w, 0x6420) ^ 0x80808080u : none;
+            // q sum = 256 sum(qh) + sum(ql) + 128 per dimension
+            const int32_t hi = __dp4a(static_cast<int>(qa[i][0]), 0x01010101, __dp4a(static_cast<int>(qa[i][2]), 0x01010101, 0));
+            const int32_t lo = __dp4a(static_cast<int>(qa[i][1]), 0x01010101, __dp4a(static_cast<int>(qa[i][3]), 0x01010101, 0));
+            v[i >> 1] += 256 * hi + lo;
+        }
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
+            v[a] += __shfl_xor_sync(~0u, v[a], 1);
+            v[a] += __shfl_xor_sync(~0u, v[a], 2);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) qc[h][a] = __shfl_sync(~0u, v[a], 4 * h) + 128 * 64;
+        }
+    }
 
     // ---------------------------------------------------------------- pass 1: scores and their maximum
-    int32_t mx[H];
+    const ScoreShift shift(p.shift_s);
+    int32_t mx[NH];
 #pragma unroll
-    for (int h = 0; h < H; ++h) mx[h] = -32768;
-    for (int t = t0 + warp; t < t1; t += nw) {
-        int id[2];
-        const uint8_t* sl[2];
-        page_ids(t, id);
-        slabs(g.k_pool, id, t, sl);
-        const int slot0 = (32 * t) & slot_mask, slot1 = (32 * t + 16) & slot_mask;
+    for (int h = 0; h < NH; ++h) mx[h] = -32768;
+    int16_t* my_scores = score_s + 32 * (first - t0) + lane;
+    const bool keeps = gid < NH || gid == 7;  // rows of heads and the row of ones
+    const int raw_row = gid < NH ? gid : NH;
+    int64_t cq[NH];
+    if constexpr (BITS == 16) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            int32_t s = 0;
+#pragma unroll
+            for (int a = 0; a < A; ++a) s += qc[h][a];
+            cq[h] = static_cast<int64_t>(s) * 128 + shift.half;
+        }
+    }
+    for (int i = 0; i < n; ++i) {
+        const uint8_t* tile = next_tile();
+        const int key = 32 * (first + (i << stride_log2)) + lane;
+        const bool in = key < len;
+        int16_t* sc = my_scores + (32 * i << stride_log2);
         if constexpr (BITS == 4) {
-            uint2 kw[A][4];
-            uint32_t sw[A];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const uint8_t* row = sl[n >> 1] + ((n >> 1 ? slot1 : slot0) + 8 * (n & 1) + gid) * (HD / 2);
-#pragma unroll
-                for (int a = 0; a < A; ++a) kw[a][n] = *reinterpret_cast<const uint2*>(row + 32 * a + 8 * tig);
-            }
-            {
-                const uint32_t* w = reinterpret_cast<const uint32_t*>((lane < 16 ? sl[0] : sl[1]) + scale_at) +
-                                    ((lane < 16 ? slot0 : slot1) + (lane & 15)) * A;
-#pragma unroll
-                for (int a = 0; a < A; ++a) sw[a] = w[a];
-            }
-            int32_t* raw = reinterpret_cast<int32_t*>(stage);
+            int32_t* raw = reinterpret_cast<int32_t*>(temp);
 #pragma unroll
             for (int a = 0; a < A; ++a)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    int32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-                    const uint32_t l0 = kw[a][n].x & 0x0F0F0F0Fu, l1 = kw[a][n].y & 0x0F0F0F0Fu;
-                    const uint32_t h0 = (kw[a][n].x >> 4) & 0x0F0F0F0Fu, h1 = (kw[a][n].y >> 4) & 0x0F0F0F0Fu;
-                    mma_m16n8k32<true, false>(hi, qh[2 * a][0], 0, qh[2 * a][1], 0, l0, l1);
-                    mma_m16n8k32<false, false>(lo, ql[2 * a][0], 0, ql[2 * a][1], 0, l0, l1);
-                    mma_m16n8k32<true, false>(hi, qh[2 * a + 1][0], 0, qh[2 * a + 1][1], 0, h0, h1);
-                    mma_m16n8k32<false, false>(lo, ql[2 * a + 1][0], 0, ql[2 * a + 1][1], 0, h0, h1);
-                    if (gid < nh)
-                        *reinterpret_cast<int2*>(raw + (a * H + gid) * C::RAW_ROW + 8 * n + 2 * tig) =
-                            make_int2(hi[0] * 256 + lo[0], hi[1] * 256 + lo[1]);
+                for (int nn = 0; nn < 4; ++nn) {
+                    const int at = (8 * nn + gid) * C::ROW + (HD == 128 ? 32 * (a ^ (gid >> 1 & 1)) : 0) + 8 * tig;
+                    const uint2 w = *reinterpret_cast<const uint2*>(tile + at);
+                    int32_t c[4];
+                    mma_s8s8_first(c, qa[2 * a], w.x & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu);
+                    mma_s8s8(c, qa[2 * a + 1], (w.x >> 4) & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu);
+                    // (the row of ones has zeros in its first half)
+                    if (keeps)
+                        *reinterpret_cast<int2*>(raw + (a * (NH + 1) + raw_row) * C::RAW_ROW + 8 * nn + 2 * tig) =
+                            make_int2(c[0] * 256 + c[2], c[1] * 256 + c[3]);
                 }
             __syncwarp();
+            int64_t base = shift.half;
+            int32_t m[A], z[A];
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                if (h >= nh) break;
-                int64_t acc = 0;
+            for (int a = 0; a < A; ++a) {
+                const uint32_t sw = *reinterpret_cast<const uint32_t*>(tile + 32 * C::ROW + 4 * (A * lane + a));
+                m[a] = static_cast<int32_t>(sw & 0xFFFFu);
+                z[a] = static_cast<int32_t>(sw) >> 16;
+                base += static_cast<int64_t>(m[a]) * (128 * raw[(a * (NH + 1) + NH) * C::RAW_ROW + lane]);
+            }
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                int64_t acc = base;
 #pragma unroll
                 for (int a = 0; a < A; ++a)
-                    acc += static_cast<int64_t>(raw[(a * H + h) * C::RAW_ROW + lane]) * static_cast<int32_t>(sw[a] & 0xFFFFu) +
-                           static_cast<int64_t>(qs[h][a]) * (static_cast<int32_t>(sw[a]) >> 16);
-                const int32_t s = static_cast<int32_t>(sat64(rs64(acc, p.shift_s), 16));
-                score_s[h * part_cap + 32 * (t - t0) + lane] = static_cast<int16_t>(s);
-                if (32 * t + lane < len) mx[h] = max(mx[h], s);
+                    acc += static_cast<int64_t>(m[a]) * raw[(a * (NH + 1) + h) * C::RAW_ROW + lane] + static_cast<int64_t>(z[a]) * qc[h][a];
+                const int32_t s = shift(acc);
+                sc[h * part_cap] = static_cast<int16_t>(s);
+                mx[h] = max(mx[h], in ? s : -32768);
             }
         } else {
-            int64_t* raw = reinterpret_cast<int64_t*>(stage);
-            uint4 kw[C::KS][4];
+            int64_t* raw = reinterpret_cast<int64_t*>(temp);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const uint8_t* row = sl[n >> 1] + ((n >> 1 ? slot1 : slot0) + 8 * (n & 1) + gid) * (HD * 2);
+            for (int nn = 0; nn < 4; ++nn) {
+                int32_t ch[4], cl[4];
 #pragma unroll
-                for (int i = 0; i < C::KS; ++i) kw[i][n] = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * tig);
-            }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                int32_t hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < C::KS; ++i) {
-                    const uint4 w = kw[i][n];
-                    const uint32_t l0 = __byte_perm(w.x, w.y, 0x6420), l1 = __byte_perm(w.z, w.w, 0x6420);
+                for (int k = 0; k < C::KS; ++k) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(tile + (8 * nn + gid) * C::ROW + 16 * ((4 * k + tig) ^ (gid & 1) * 4));
                     const uint32_t h0 = __byte_perm(w.x, w.y, 0x7531), h1 = __byte_perm(w.z, w.w, 0x7531);
-                    mma_m16n8k32<true, true>(hh, qh[i][0], 0, qh[i][1], 0, h0, h1);
-                    mma_m16n8k32<true, false>(mid, qh[i][0], 0, qh[i][1], 0, l0, l1);
-                    mma_m16n8k32<false, true>(mid, ql[i][0], 0, ql[i][1], 0, h0, h1);
-                    mma_m16n8k32<false, false>(ll, ql[i][0], 0, ql[i][1], 0, l0, l1);
+                    const uint32_t l0 = __byte_perm(w.x, w.y, 0x6420) ^ 0x80808080u, l1 = __byte_perm(w.z, w.w, 0x6420) ^ 0x80808080u;
+                    if (k == 0) {
+                        mma_s8s8_first(ch, qa[k], h0, h1);
+                        mma_s8s8_first(cl, qa[k], l0, l1);
+                    } else {
+                        mma_s8s8(ch, qa[k], h0, h1);
+                        mma_s8s8(cl, qa[k], l0, l1);
+                    }
                 }
-                if (gid < nh) {
-                    int64_t* o = raw + gid * C::RAW_ROW + 8 * n + 2 * tig;
+                // heads: 65536 qh.kh + 256 (ql.kh + qh.kl) + ql.kl; ones: 256 sum(kh) + sum(kl)
+                if (keeps)
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
-                        o[c] = static_cast<int64_t>(hh[c]) * 65536 + static_cast<int64_t>(mid[c]) * 256 + ll[c];
-                }
+                        raw[raw_row * C::RAW_ROW + 8 * nn + 2 * tig + c] =
+                            static_cast<int64_t>(ch[c]) * 65536 + (static_cast<int64_t>(ch[2 + c] + cl[c]) * 256 + cl[2 + c]);
             }
             __syncwarp();
+            const int64_t ck = raw[NH * C::RAW_ROW + lane] * 128;
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                if (h >= nh) break;
-                const int32_t s = static_cast<int32_t>(sat64(rs64(raw[h * C::RAW_ROW + lane], p.shift_s), 16));
-                score_s[h * part_cap + 32 * (t - t0) + lane] = static_cast<int16_t>(s);
-                if (32 * t + lane < len) mx[h] = max(mx[h], s);
+            for (int h = 0; h < NH; ++h) {
+                const int32_t s = shift(raw[h * C::RAW_ROW + lane] + ck + cq[h]);
+                sc[h * part_cap] = static_cast<int16_t>(s);
+                mx[h] = max(mx[h], in ? s : -32768);
             }
         }
-        __syncwarp();
     }
-    __syncthreads();  // the block's tables and reduction words are set
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        const int32_t m = __reduce_max_sync(~0u, mx[h]);
-        if (lane == 0) atomicMax(&max_s[h], m);
-    }
-    if (cs > 1) {
-        cluster_barrier();
+    for (int h = 0; h < NH; ++h) mx[h] = __reduce_max_sync(~0u, mx[h]);
+    if constexpr (!WARP) {
+        if (lane == 0)
 #pragma unroll
-        for (int h = 0; h < H; ++h)
-            mx[h] = __reduce_max_sync(~0u, lane < cs ? ld_remote32(remote_smem(&max_s[h], lane)) : -32768);
-    } else {
+            for (int h = 0; h < NH; ++h) max_s[h][warp] = mx[h];
         __syncthreads();
 #pragma unroll
-        for (int h = 0; h < H; ++h) mx[h] = max_s[h];
+        for (int h = 0; h < NH; ++h) mx[h] = __reduce_max_sync(~0u, lane < nw ? max_s[h][lane] : -32768);
+        if (cs > 1) {
+            if (tid == 0)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) max_s[h][PATTN_MAX_WARPS] = mx[h];
+            cluster_barrier();
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+                mx[h] = __reduce_max_sync(~0u, lane < cs ? ld_remote32(remote_smem(&max_s[h][PATTN_MAX_WARPS], lane)) : -32768);
+        }
     }
 
     // ---------------------------------------------------------------- pass 2: sum of the exponentials
-    {
-        unsigned long long z[H];
+    uint64_t z[NH];
 #pragma unroll
-        for (int h = 0; h < H; ++h) z[h] = 0;
-        for (int t = t0 + warp; t < t1; t += nw)
-            if (32 * t + lane < len)
+    for (int h = 0; h < NH; ++h) z[h] = 0;
+    for (int i = 0; i < n; ++i) {
+        const bool in = 32 * (first + (i << stride_log2)) + lane < len;
+        const int16_t* sc = my_scores + (32 * i << stride_log2);
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    if (h >= nh) break;
-                    const int32_t d = mx[h] - score_s[h * part_cap + 32 * (t - t0) + lane];
-                    z[h] += d > PAGED_DMAX ? 0 : exp_s[d];
-                }
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            // in pieces of 24 and 32 bits: 32 lanes of 2^24 and of 2^47 / 2^24 stay in 32 bits
-            const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(z[h]) & 0xFFFFFFu);
-            const uint32_t hi = __reduce_add_sync(~0u, static_cast<uint32_t>(z[h] >> 24));
-            if (lane == 0) atomicAdd(&z_s[h], (static_cast<unsigned long long>(hi) << 24) + lo);
+        for (int h = 0; h < NH; ++h) {
+            const int d = in ? min(mx[h] - sc[h * part_cap], PAGED_DMAX + 1) : PAGED_DMAX + 1;
+            z[h] += static_cast<uint32_t>(exp_s[d]);
         }
     }
-    uint64_t z[H];
-    if (cs > 1) {
-        cluster_barrier();
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const uint64_t v = lane < cs ? static_cast<uint64_t>(ld_remote64(remote_smem(&z_s[h], lane))) : 0;
-            const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(v) & 0xFFFFFFu);
-            const uint32_t hi = __reduce_add_sync(~0u, static_cast<uint32_t>(v >> 24));
-            z[h] = (static_cast<uint64_t>(hi) << 24) + lo;
-        }
-    } else {
+    for (int h = 0; h < NH; ++h) z[h] = warp_sum47(z[h]);
+    if constexpr (!WARP) {
+        if (lane == 0)
+#pragma unroll
+            for (int h = 0; h < NH; ++h) z_s[h][warp] = z[h];
         __syncthreads();
 #pragma unroll
-        for (int h = 0; h < H; ++h) z[h] = z_s[h];
+        for (int h = 0; h < NH; ++h) z[h] = warp_sum47(lane < nw ? z_s[h][lane] : 0);
+        if (cs > 1) {
+            if (tid == 0)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) z_s[h][PATTN_MAX_WARPS] = z[h];
+            cluster_barrier();
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+                z[h] = warp_sum47(lane < cs ? static_cast<uint64_t>(ld_remote64(remote_smem(&z_s[h][PATTN_MAX_WARPS], lane))) : 0);
+        }
     }
 
     // ---------------------------------------------------------------- pass 3: probabilities times V
-    float zscale[H];
+    uint32_t rcp[NH];
+    {
+        uint64_t d = z[0];
 #pragma unroll
-    for (int h = 0; h < H; ++h) zscale[h] = __fdiv_rn(static_cast<float>(1 << p.prob_bits), static_cast<float>(z[h]));
-    // key lane of a tile -> its byte of a plane row, so that a thread's 8 bytes are keys tig + 4 i + 16 h
-    const int plane_at = 8 * (lane & 3) + 4 * (lane >> 4) + ((lane >> 2) & 3);
+        for (int h = 1; h < NH; ++h) d = lane == h ? z[h] : d;
+        const uint32_t q = static_cast<uint32_t>((1ull << 61) / d);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) rcp[h] = __shfl_sync(~0u, q, h);
+    }
+    // key lane of a tile -> its word of a weight row, so that a thread's 8 words are keys tig + 4 i + 16 k
+    uint32_t* wgt = reinterpret_cast<uint32_t*>(temp);
+    uint32_t* my_wgt = wgt + 8 * (lane & 3) + 4 * (lane >> 4) + ((lane >> 2) & 3);
+    const uint32_t byte_sel = (gid & 3) * 0x11 + 0x40;
+    if (NH < 2 * C::RR) {  // rows of heads that are never there
+        __syncwarp();
+        for (int i = lane; i < C::WGT_BYTES / 4; i += 32) wgt[i] = 0;
+    }
+#pragma unroll 1
     for (int sweep = 0; sweep < C::SWEEPS; ++sweep) {
         int32_t acc[C::NT][4];
 #pragma unroll
         for (int i = 0; i < C::NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
-        int64_t pz[H][A];
+        int64_t pz[NH][A];
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+        for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int a = 0; a < A; ++a) pz[h][a] = 0;
-        if (nh < H)
-            for (int i = lane; i < C::PLANE_BYTES / 4; i += 32) reinterpret_cast<uint32_t*>(stage)[i] = 0;  // absent heads
-        __syncwarp();
-        for (int t = t0 + warp; t < t1; t += nw) {
-            int id[2];
-            const uint8_t* sl[2];
-            page_ids(t, id);
-            slabs(g.v_pool, id, t, sl);
-            const int slot0 = (32 * t) & slot_mask, slot1 = (32 * t + 16) & slot_mask;
-            uint32_t vw[BITS == 4 ? A : 4][8];  // [group or word][key tig + 4 i (+ 16)]
-            uint32_t sw[A];
+        for (int i = 0; i < n; ++i) {
+            const uint8_t* tile = next_tile();
+            const bool in = 32 * (first + (i << stride_log2)) + lane < len;
+            const int16_t* sc = my_scores + (32 * i << stride_log2);
+            uint32_t e[NH], pr[NH];
+            bool unsure = false;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int slot = (i < 4 ? slot0 : slot1) + tig + 4 * (i & 3);
-                if constexpr (BITS == 4) {
-#pragma unroll
-                    for (int a = 0; a < A; ++a)
-                        vw[a][i] = *reinterpret_cast<const uint32_t*>(sl[i >> 2] + slot * (HD / 2) + 32 * a + 4 * gid);
-                } else {
-                    const uint4 w = *reinterpret_cast<const uint4*>(sl[i >> 2] + slot * (HD * 2) + 128 * sweep + 16 * gid);
-                    vw[0][i] = w.x; vw[1][i] = w.y; vw[2][i] = w.z; vw[3][i] = w.w;
-                }
+            for (int h = 0; h < NH; ++h) {
+                const int d = in ? min(mx[h] - sc[h * part_cap], PAGED_DMAX + 1) : PAGED_DMAX + 1;
+                e[h] = static_cast<uint32_t>(exp_s[d]);
+                pr[h] = prob_of(e[h], p.prob_bits, rcp[h], unsure);
             }
+            if (unsure)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) pr[h] = prob_exact(pr[h], e[h], p.prob_bits, z[h]);
             if constexpr (BITS == 4) {
-                const uint32_t* w = reinterpret_cast<const uint32_t*>((lane < 16 ? sl[0] : sl[1]) + scale_at) +
-                                    ((lane < 16 ? slot0 : slot1) + (lane & 15)) * A;
 #pragma unroll
-                for (int a = 0; a < A; ++a) sw[a] = w[a];
-            }
+                for (int a = 0; a < A; ++a) {
+                    const uint32_t sw = *reinterpret_cast<const uint32_t*>(tile + 32 * C::ROW + 4 * (A * lane + a));
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                if (h >= nh) break;
-                uint32_t pr = 0;
-                if (32 * t + lane < len) {
-                    const int32_t d = mx[h] - score_s[h * part_cap + 32 * (t - t0) + lane];
-                    if (d <= PAGED_DMAX) pr = prob_of(exp_s[d], p.prob_bits, z[h], zscale[h]);
-                }
-                if constexpr (BITS == 4) {
-#pragma unroll
-                    for (int a = 0; a < A; ++a) {
-                        const uint32_t w = pr * (sw[a] & 0xFFFFu);
-                        pz[h][a] += static_cast<int64_t>(static_cast<int32_t>(pr)) * (static_cast<int32_t>(sw[a]) >> 16);
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) stage[a * 512 + (h * 4 + b) * 32 + plane_at] = static_cast<uint8_t>(w >> (8 * b));
+                    for (int h = 0; h < NH; ++h) {
+                        pz[h][a] += static_cast<int64_t>(static_cast<int32_t>(pr[h])) * (static_cast<int32_t>(sw) >> 16);
+                        my_wgt[(a * 2 * C::RR + h) * 32] = pr[h] * (sw & 0xFFFFu);
                     }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) stage[(h * 4 + b) * 32 + plane_at] = static_cast<uint8_t>(pr >> (8 * b));
                 }
+            } else {
+#pragma unroll
+                for (int h = 0; h < NH; ++h) my_wgt[h * 32] = pr[h];
             }
             __syncwarp();
 #pragma unroll
             for (int a = 0; a < C::GPS; ++a) {
-                const uint2 x = *reinterpret_cast<const uint2*>(stage + (BITS == 4 ? a * 512 : 0) + gid * 32 + 8 * tig);
-                const uint2 y = *reinterpret_cast<const uint2*>(stage + (BITS == 4 ? a * 512 : 0) + (gid + 8) * 32 + 8 * tig);
+                uint32_t x[4] = {0, 0, 0, 0};  // rows gid and gid + 8: one byte of eight keys' weights
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int rr = 0; rr < C::RR; ++rr) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(wgt + (a * 2 * C::RR + (gid >> 2) + 2 * rr) * 32 + 8 * tig + 4 * k);
+                        x[rr + 2 * k] = __byte_perm(__byte_perm(w.x, w.y, byte_sel), __byte_perm(w.z, w.w, byte_sel), 0x5410);
+                    }
                 if constexpr (BITS == 4) {
-                    uint32_t b0[4], b1[4];
-                    transpose4(vw[a][0], vw[a][1], vw[a][2], vw[a][3], b0);
-                    transpose4(vw[a][4], vw[a][5], vw[a][6], vw[a][7], b1);
+                    uint32_t w[8], b0[4], b1[4];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int row = tig + 4 * k;  // (keys tig + 4 i and, from k = 4, 16 further on)
+                        w[k] = *reinterpret_cast<const uint32_t*>(tile + row * C::ROW + (HD == 128 ? 32 * (a ^ (row >> 1 & 1)) : 0) + 4 * gid);
+                    }
+                    transpose4(w[0], w[1], w[2], w[3], b0);
+                    transpose4(w[4], w[5], w[6], w[7], b1);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        mma_m16n8k32<false, false>(acc[8 * a + 2 * j], x.x, y.x, x.y, y.y, b0[j] & 0x0F0F0F0Fu, b1[j] & 0x0F0F0F0Fu);
-                        mma_m16n8k32<false, false>(acc[8 * a + 2 * j + 1], x.x, y.x, x.y, y.y, (b0[j] >> 4) & 0x0F0F0F0Fu,
-                                                   (b1[j] >> 4) & 0x0F0F0F0Fu);
+                        mma_u8u8(acc[8 * a + 2 * j], x, b0[j] & 0x0F0F0F0Fu, b1[j] & 0x0F0F0F0Fu);
+                        mma_u8u8(acc[8 * a + 2 * j + 1], x, (b0[j] >> 4) & 0x0F0F0F0Fu, (b1[j] >> 4) & 0x0F0F0F0Fu);
                     }
                 } else {
+                    uint4 w[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t b0[4], b1[4];
-                        transpose4(vw[j][0], vw[j][1], vw[j][2], vw[j][3], b0);
-                        transpose4(vw[j][4], vw[j][5], vw[j][6], vw[j][7], b1);
-                        mma_m16n8k32<false, false>(acc[4 * j + 0], x.x, y.x, x.y, y.y, b0[0], b1[0]);
-                        mma_m16n8k32<false, true>(acc[4 * j + 1], x.x, y.x, x.y, y.y, b0[1], b1[1]);
-                        mma_m16n8k32<false, false>(acc[4 * j + 2], x.x, y.x, x.y, y.y, b0[2], b1[2]);
-                        mma_m16n8k32<false, true>(acc[4 * j + 3], x.x, y.x, x.y, y.y, b0[3], b1[3]);
+                    for (int k = 0; k < 8; ++k) {
+                        const int row = tig + 4 * k;
+                        w[k] = *reinterpret_cast<const uint4*>(tile + row * 128 + 16 * (gid ^ 2 * tig));
                     }
+                    auto four = [&](int j, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4, uint32_t w5, uint32_t w6, uint32_t w7) {
+                        uint32_t b0[4], b1[4];
+                        transpose4(w0, w1, w2, w3, b0);
+                        transpose4(w4, w5, w6, w7, b1);
+                        mma_u8u8(acc[4 * j + 0], x, b0[0], b1[0]);
+                        mma_u8s8(acc[4 * j + 1], x, b0[1], b1[1]);
+                        mma_u8u8(acc[4 * j + 2], x, b0[2], b1[2]);
+                        mma_u8s8(acc[4 * j + 3], x, b0[3], b1[3]);
+                    };
+                    four(0, w[0].x, w[1].x, w[2].x, w[3].x, w[4].x, w[5].x, w[6].x, w[7].x);
+                    four(1, w[0].y, w[1].y, w[2].y, w[3].y, w[4].y, w[5].y, w[6].y, w[7].y);
+                    four(2, w[0].z, w[1].z, w[2].z, w[3].z, w[4].z, w[5].z, w[6].z, w[7].z);
+                    four(3, w[0].w, w[1].w, w[2].w, w[3].w, w[4].w, w[5].w, w[6].w, w[7].w);
                 }
             }
+        }
+        // Accumulators to shared memory: word 8 i + column of row 4 h + b, joined over the block's warps (255 x
+        // 255 x PATTN_MAX_PART stays in 32 bits).  Four rows are skewed by a word against bank conflicts.
+        if constexpr (WARP) {
+            if (sweep + 1 == C::SWEEPS) cp_async_wait<0>();  // (the ring's copies have ended; the last ones are empty)
             __syncwarp();
         }
-        // join the warps: 255 x 255 x PATTN_MAX_PART stays in 32 bits
-        if (t0 + warp < t1) {
+        int32_t* warp_acc = WARP && C::SWEEPS > 1 ? nullptr : acc_s;
+        if (WARP && C::SWEEPS > 1) warp_acc = reinterpret_cast<int32_t*>(score_s + NH * part_cap);
+        if (n > 0) {
+            int32_t* at = warp_acc + gid * C::ACC_LD + (gid >> 2) + 2 * tig;
 #pragma unroll
-            for (int i = 0; i < C::NT; ++i)
+            for (int rr = 0; rr < C::RR; ++rr)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int col = 2 * tig + (c & 1);
-                    const int at = BITS == 4 ? 64 * (i >> 3) + 4 * col + ((i & 7) >> 1) + 32 * (i & 1)
-                                             : 64 * (i & 1) + 8 * col + 2 * (i >> 2) + ((i >> 1) & 1);
-                    if ((gid + 8 * (c >> 1)) < 4 * nh) atomicAdd(&acc_s[(gid + 8 * (c >> 1)) * C::ACC_LD + at], acc[i][c]);
-                }
-            if constexpr (BITS == 4) {
+                for (int i = 0; i < C::NT; ++i)
 #pragma unroll
-                for (int h = 0; h < H; ++h)
-#pragma unroll
-                    for (int a = 0; a < A; ++a) {
-                        const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(pz[h][a]) & 0xFFFFFFu);
-                        const int32_t hi = __reduce_add_sync(~0u, static_cast<int32_t>(pz[h][a] >> 24));
-                        if (lane == 0) {
-                            atomicAdd(&zlo_s[h * A + a], lo);
-                            atomicAdd(&zhi_s[h * A + a], hi);
-                        }
+                    for (int c = 0; c < 2; ++c) {
+                        int32_t* o = at + rr * (8 * C::ACC_LD + 2) + 8 * i + c;
+                        if constexpr (WARP) *o = acc[i][2 * rr + c];
+                        else atomicAdd(o, acc[i][2 * rr + c]);
                     }
-            }
         }
-        __syncthreads();
-        for (int i = tid; i < nh * 64 * C::GPS; i += blockDim.x) {
-            const int h = i / (64 * C::GPS), d = i % (64 * C::GPS);
-            int64_t v = 0;
+        if constexpr (BITS == 4) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                int32_t* x = acc_s + (4 * h + b) * C::ACC_LD + d;
-                int64_t y = x[0];
-                if constexpr (BITS == 16) {
-                    y += static_cast<int64_t>(x[64]) * 256;
-                    if (sweep + 1 < C::SWEEPS) x[0] = x[64] = 0;
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int a = 0; a < A; ++a) {
+                    pz[h][a] = warp_sum_signed(pz[h][a]);
+                    if (!WARP && lane == 0) pz_s[h * A + a][warp] = pz[h][a];
                 }
-                v += y << (8 * b);
+        }
+        if constexpr (WARP) __syncwarp();
+        else __syncthreads();
+        if constexpr (BITS == 4 && !WARP) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int a = 0; a < A; ++a) pz[h][a] = warp_sum_signed(lane < nw ? pz_s[h * A + a][lane] : 0);
+        }
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            if (h >= nh) break;
+            for (int d = me; d < 64 * C::GPS; d += team) {
+                // 4 bits: dimension 32 k + 4 n + j of a group is column n of tile 2 j + k; 16 bits: dimension 8 n + d'
+                // has its bytes in column n of tiles 2 d' and 2 d' + 1
+                const int word = BITS == 4 ? 64 * (d >> 6) + 16 * (d & 3) + 8 * ((d >> 5) & 1) + ((d >> 2) & 7) : 16 * (d & 7) + (d >> 3);
+                int64_t v = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    int32_t* x = warp_acc + (4 * h + b) * C::ACC_LD + h + word;
+                    int64_t y = x[0];
+                    if constexpr (BITS == 16) {
+                        y += static_cast<int64_t>(x[8]) * 256;
+                        if (!WARP && sweep + 1 < C::SWEEPS) x[0] = x[8] = 0;
+                    }
+                    v += y << (8 * b);
+                }
+                if constexpr (BITS == 4) v += A == 1 || d < 64 ? pz[h][0] : pz[h][A - 1];
+                if (!WARP && cs > 1) ctx_s[h * HD + 64 * sweep + d] = v;
+                else ctx[h * HD + 64 * sweep + d] = static_cast<int32_t>(sat64(rs64(v, p.shift_c), p.bits_c));
             }
-            if constexpr (BITS == 4)
-                v += static_cast<int64_t>(zlo_s[h * A + (d >> 6)]) + (static_cast<int64_t>(zhi_s[h * A + (d >> 6)]) << 24);
-            if (cs > 1) ctx_s[h * HD + 64 * sweep + d] = v;
-            else ctx[h * HD + 64 * sweep + d] = static_cast<int32_t>(sat64(rs64(v, p.shift_c), p.bits_c));
         }
-        if (sweep + 1 < C::SWEEPS) __syncthreads();
+        if (!WARP && sweep + 1 < C::SWEEPS) __syncthreads();
+        if (WARP && sweep + 1 < C::SWEEPS) __syncwarp();
     }
-    if (cs > 1) {
-        cluster_barrier();
-        for (int i = rank * blockDim.x + tid; i < nh * HD; i += cs * blockDim.x) {
-            int64_t v = 0;
-            for (int c = 0; c < cs; ++c) v += ld_remote64(remote_smem(ctx_s + i, c));
-            ctx[i] = static_cast<int32_t>(sat64(rs64(v, p.shift_c), p.bits_c));
+    if constexpr (!WARP) {
+        if (cs > 1) {
+            cluster_barrier();
+            for (int i = rank * blockDim.x + tid; i < nh * HD; i += cs * blockDim.x) {
+                int64_t v = 0;
+                for (int c = 0; c < cs; ++c) v += ld_remote64(remote_smem(ctx_s + i, c));
+                ctx[i] = static_cast<int32_t>(sat64(rs64(v, p.shift_c), p.bits_c));
+            }
+            cluster_barrier();  // no block leaves while its words are read
         }
-        cluster_barrier();  // no block leaves while its words are read
     }
 }
 

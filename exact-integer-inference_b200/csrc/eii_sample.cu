@@ -41,14 +41,14 @@ int eii_sample(eii_sampler* s, const int32_t* logits, int64_t ld, int n_rows, in
                const int32_t* top_k, const int32_t* top_p, const int32_t* min_p, const uint32_t* u, int64_t* token,
                int32_t* kept, int32_t* prob, void* stream) {
     if (!s) return fail(EII_ERR_ARG, "sampler is null");
-    if (!logits || !u || !token) return fail(EII_ERR_ARG, "logits, u or token is null");
     if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (n_rows == 0) return EII_OK;
+    if (!logits || !u || !token) return fail(EII_ERR_ARG, "logits, u or token is null");
     if (vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return fail(EII_ERR_ARG, "vocab must be in [1, %d] (got %d)", SAMPLE_MAX_VOCAB, vocab);
     if (ld < vocab) return fail(EII_ERR_ARG, "ld must be >= %d (got %lld)", vocab, (long long)ld);
     if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(u)) & 3)
         return fail(EII_ERR_ARG, "logits and u must be 4-byte aligned");
     if (reinterpret_cast<uintptr_t>(token) & 7) return fail(EII_ERR_ARG, "token must be 8-byte aligned");
-    if (n_rows == 0) return EII_OK;
     DeviceGuard dg(s->device);
     CK(dg.st);
     SampleParams p{};

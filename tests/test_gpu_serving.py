@@ -140,6 +140,8 @@ def test_append_without_q_in_place_and_default_sequences(torch):
     c.check_pools()
     assert np.array_equal(d[0].cpu().numpy(), wq)
     c.p.append(c.pages, d[1].data_ptr(), d[2].data_ptr(), 0, dpos.data_ptr(), 30, stream=st(torch))
+    c.p.append(c.pages, None, None, 0, None, 30, stream=st(torch))  # (an empty tensor's pointer)
+    c.p.attention(c.pages, None, 0, None, 512, 17, 16, 16, None, stream=st(torch))
     c.p.sync(st(torch))
     c.check_pools()
 
@@ -444,6 +446,7 @@ def test_sampling_refusals(torch, sampler):
         assert tok.tolist() == [0, -1]
         sampler.sync(st(torch))
     call(n=0)
+    sampler.sample(None, 0, 64, None, None, stream=st(torch))
     sampler.sync(st(torch))
 
 
