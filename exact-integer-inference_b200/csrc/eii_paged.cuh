@@ -10,6 +10,7 @@
 #pragma once
 #include <cstdint>
 
+#include "eii_cluster.cuh"
 #include "eii_int.cuh"
 #include "eii_ptx.cuh"
 
@@ -207,13 +208,6 @@ struct PattnCfg {
     }
 };
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // D = A B (+ D) on 16 x 8 x 32 bytes: A rows are query heads (scores) or head x weight byte (context), B
 // columns are keys or dimensions.  A decoding step has a handful of rows, so the 128-row tcgen05 tile
 // would be empty: the warp-level instruction takes its operands from registers, straight from the loads.
@@ -272,42 +266,6 @@ __device__ __forceinline__ uint32_t prob_of(uint32_t e, int pb, uint32_t rcp, bo
 __device__ __forceinline__ uint32_t prob_exact(uint32_t q, uint32_t e, int pb, uint64_t z) {
     const int64_t rem = static_cast<int64_t>((static_cast<uint64_t>(e) << pb) + (z >> 1) - q * z);
     return rem < 0 ? q - 1 : rem >= static_cast<int64_t>(z) ? q + 1 : q;
-}
-
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t remote_smem(const void* p, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ int32_t ld_remote32(uint32_t a) {
-    int32_t v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ int64_t ld_remote64(uint32_t a) {
-    int64_t v;
-    asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-    return v;
-}
-// Sum of a non-negative v < 2^47 over the warp, in pieces of 24 and 23 bits.
-__device__ __forceinline__ uint64_t warp_sum47(uint64_t v) {
-    const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(v) & 0xFFFFFFu);
-    const uint32_t hi = __reduce_add_sync(~0u, static_cast<uint32_t>(v >> 24));
-    return (static_cast<uint64_t>(hi) << 24) + lo;
-}
-// The same of a signed |v| < 2^50.
-__device__ __forceinline__ int64_t warp_sum_signed(int64_t v) {
-    const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(v) & 0xFFFFFFu);
-    const int32_t hi = __reduce_add_sync(~0u, static_cast<int32_t>(v >> 24));
-    return (static_cast<int64_t>(hi) << 24) + lo;
 }
 
 // An item is (row, kv head, up to NH query heads).  WARP: one warp works on an item by itself (many

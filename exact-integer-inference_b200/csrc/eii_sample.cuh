@@ -11,6 +11,9 @@
 #pragma once
 #include <cstdint>
 
+#include <type_traits>
+
+#include "eii_cluster.cuh"
 #include "eii_int.cuh"
 
 namespace eii {
@@ -52,18 +55,17 @@ __device__ __forceinline__ SampleRow sample_row(const SampleParams& p, int r) {
     return o;
 }
 
-// floor(y f / 2^31) of the 31-bit fraction f is umulhi(y, 2 f).
+// floor(y f / 2^31) of the 31-bit fraction f is umulhi(y, 2 f); RS(y, n) = ((2 y >> n) + 1) >> 1.
 __device__ __forceinline__ uint32_t sample_weight(int32_t l, int32_t row_max, uint32_t b2) {
-    if (l == SAMPLE_MASKED) return 0;
     const uint64_t x = static_cast<uint64_t>(static_cast<uint32_t>(row_max) - static_cast<uint32_t>(l)) * b2;
-    const uint32_t n = static_cast<uint32_t>(x >> 40);
-    if (n > 30) return 0;
-    const uint32_t f2 = static_cast<uint32_t>(x >> 8) & 0xFFFFFF00u;
+    const uint32_t hi = static_cast<uint32_t>(x >> 32);
+    const uint32_t f2 = __funnelshift_r(static_cast<uint32_t>(x), hi, 8) & 0xFFFFFF00u;
     uint32_t y = SAMPLE_C3 - __umulhi(SAMPLE_C4, f2);
     y = SAMPLE_C2 - __umulhi(y, f2);
     y = SAMPLE_C1 - __umulhi(y, f2);
-    y = (1u << 30) - __umulhi(y, f2);
-    return (y + ((1u << n) >> 1)) >> n;
+    y = (1u << 31) - 2 * __umulhi(y, f2);
+    const uint32_t w = (__funnelshift_rc(y, 0, hi >> 8) + 1) >> 1;
+    return hi < (31u << 8) && l != SAMPLE_MASKED ? w : 0;
 }
 
 // ceil(p mass / 2^16), at least 1.
@@ -76,124 +78,513 @@ __device__ __forceinline__ uint64_t sample_target(uint64_t mass, uint32_t u) {
     return (u * (mass >> 24) + ((u * (mass & 0xFFFFFF)) >> 24)) >> 8;
 }
 
-constexpr int SAMPLE_THREADS = 256;
+// ------------------------------------------------------------------------------------------ kernel
+// A cluster of `cs` blocks per row, the row's weights in shared memory from the one time it is read: a thread
+// owns 4 ch consecutive ones (index order is block, thread, chunk of four, word).  The grid is persistent.
+//
+// The kept tokens are a prefix of the order (weight descending, index ascending): all weights above theta
+// and the first `quota` of those equal to it.  A cut is found by narrowing a window [lo, hi) around it:
+// with passes over the row, the first two at places that a sample of the row suggests, until the window is
+// short enough for a list; with passes over that list; and, from SAMPLE_FEW on, by comparing each with all.
+// Every decision rests on exact sums; the sample only chooses where to look.  A list that holds all kept
+// weights serves the draw too.
+constexpr int SAMPLE_THREADS = 1024, SAMPLE_WARPS = SAMPLE_THREADS / 32;
+constexpr int SAMPLE_MAX_CLUSTER = 16, SAMPLE_MAX_CHUNKS = 12;
+constexpr int SAMPLE_GUESS_CHUNKS = 6;
+constexpr int SAMPLE_LIST = 4096, SAMPLE_FEW = 64;
+constexpr uint32_t SAMPLE_TOP = (1u << 30) + 1;  // above every weight
 
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, unsigned long long* s) {
-    __syncthreads();
-    if (threadIdx.x == 0) *s = 0;
-    __syncthreads();
-    atomicAdd(s, static_cast<unsigned long long>(v));
-    __syncthreads();
-    return *s;
-}
+// Words that the threads of a block (and the blocks of a cluster) exchange come in two sets that take turns,
+// so that one is not overwritten before its slowest reader has it: a barrier lies between the uses of a set.
+struct SampleShared {
+    uint32_t w[SAMPLE_LIST], i[SAMPLE_LIST];  // the list; of a cluster's blocks the first half, the second for all
+    alignas(8) uint32_t few[SAMPLE_FEW];
+    int32_t warp_max[2][SAMPLE_WARPS];
+    uint64_t warp_mass[2][SAMPLE_WARPS];
+    uint32_t warp_n[2][SAMPLE_WARPS];
+    int32_t block_max[2];
+    uint64_t block_mass[2];
+    uint32_t block_n[2];
+    uint32_t few_n, theta, above_n;
+    uint64_t above;
+};
+static_assert(SAMPLE_MAX_CHUNKS * 16 * SAMPLE_THREADS + sizeof(SampleShared) <= 227 * 1024, "shared memory");
 
-// One block per row.  The kept tokens are a prefix of the order (weight descending, index ascending):
-// all weights above theta and the first `quota` of those equal to it.  Both cuts are found by bisection.
-__global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(const SampleParams p) {
-    __shared__ unsigned long long sum_s;
-    __shared__ int32_t max_s;
-    __shared__ unsigned long long mass_t[SAMPLE_THREADS];
-    __shared__ int ties_t[SAMPLE_THREADS];
-    const int r = blockIdx.x, tid = threadIdx.x, V = p.vocab;
-    const int32_t* row = p.logits + r * p.ld;
-    const SampleRow q = sample_row(p, r);
-    if (tid == 0) max_s = SAMPLE_MASKED;
-    __syncthreads();
-    int32_t mx = SAMPLE_MASKED;
-    for (int i = tid; i < V; i += SAMPLE_THREADS) mx = max(mx, row[i]);
-    atomicMax(&max_s, mx);
-    __syncthreads();
-    mx = max_s;
-    if (!q.ok || mx == SAMPLE_MASKED) {
-        if (tid == 0) {
-            if (!q.ok) atomicCAS(p.err, 0, ERR_SAMPLE_PARAM);
-            p.token[r] = -1;
-            if (p.kept) p.kept[r] = 0;
-            if (p.prob) p.prob[r] = 0;
-        }
-        return;
-    }
-    auto count_from = [&](uint32_t th) {
-        uint64_t c = 0;
-        for (int i = tid; i < V; i += SAMPLE_THREADS) c += sample_weight(row[i], mx, q.b2) >= th;
-        return block_sum(c, &sum_s);
+__global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams p, const int cs, const int ch, const int aligned) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    SampleShared& sh = *reinterpret_cast<SampleShared*>(smem + ch * 16 * SAMPLE_THREADS);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = cs > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int base = (rank * SAMPLE_THREADS + tid) * 4 * ch;  // this thread's first logit
+    const int step = gridDim.x / cs;
+    // A thread's chunk k lies at (k + shift) mod ch of its ch places: where ch is even, eight neighbours start on
+    // eight banks.
+    auto shift_of = [&](int l) {
+        int x = ch & 1 ? 0 : l & 7;
+        while (x >= ch) x -= ch;
+        return x;
     };
-    auto mass_from = [&](uint32_t th) {
-        uint64_t c = 0;
-        for (int i = tid; i < V; i += SAMPLE_THREADS) {
-            const uint32_t w = sample_weight(row[i], mx, q.b2);
-            c += w >= th ? w : 0;
+    const int shift = shift_of(lane);
+    uint4* warp_buf = reinterpret_cast<uint4*>(smem) + warp * 32 * ch;
+    uint4* buf = warp_buf + lane * ch;
+    int turn = 0;
+
+    // f(chunk's number, its place) over this thread's chunks, in index order
+    auto each = [&](auto f) {
+        int place = shift;
+#pragma unroll 4
+        for (int k = 0; k < ch; ++k) {
+            f(k, buf + place);
+            place = place + 1 == ch ? 0 : place + 1;
         }
-        return block_sum(c, &sum_s);
     };
-    uint32_t theta = 1;
-    uint64_t quota = UINT32_MAX;
-    if (q.k > 0 && count_from(1) > q.k) {
-        uint32_t lo = 1, hi = (1u << 30) + 1;  // count_from(lo) >= k > count_from(hi)
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (count_from(mid) >= q.k) lo = mid;
-            else hi = mid;
-        }
-        theta = lo;
-        quota = q.k - count_from(theta + 1);
-    }
-    if ((static_cast<uint32_t>(q.mp) << 14) > theta) {
-        theta = static_cast<uint32_t>(q.mp) << 14;
-        quota = UINT32_MAX;
-    }
-    uint64_t above = mass_from(theta + 1);
-    uint64_t equal = count_from(theta) - count_from(theta + 1);
-    if (quota > equal) quota = equal;
-    if (q.p < 65536) {
-        const uint64_t goal = sample_goal(above + quota * theta, q.p);
-        if (above >= goal) {
-            uint32_t lo = theta, hi = (1u << 30) + 1;  // mass_from(lo + 1) or its part >= goal > mass_from(hi)
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (mass_from(mid) >= goal) lo = mid;
-                else hi = mid;
-            }
-            theta = lo;
-            above = mass_from(theta + 1);
-        }
-        quota = (goal - above + theta - 1) / theta;
-    }
-    const uint64_t mass = above + quota * theta, target = sample_target(mass, p.u[r]);
-    const uint64_t above_n = count_from(theta + 1);
-    // index order: thread t owns a contiguous part
-    const int part = (V + SAMPLE_THREADS - 1) / SAMPLE_THREADS, i0 = min(tid * part, V), i1 = min(i0 + part, V);
-    uint64_t m = 0;
-    int ties = 0;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t w = sample_weight(row[i], mx, q.b2);
-        m += w > theta ? w : 0;
-        ties += w == theta;
-    }
-    mass_t[tid] = m;
-    ties_t[tid] = ties;
-    __syncthreads();
-    uint64_t run = 0, tied = 0;
-    for (int t = 0; t < tid; ++t) {
-        const uint64_t take = tied >= quota ? 0 : min(static_cast<uint64_t>(ties_t[t]), quota - tied);
-        run += mass_t[t] + take * theta;
-        tied += ties_t[t];
-    }
-    const uint64_t take = tied >= quota ? 0 : min(static_cast<uint64_t>(ties), quota - tied);
-    if (run <= target && target < run + m + take * theta) {
-        for (int i = i0; i < i1; ++i) {
-            const uint32_t w = sample_weight(row[i], mx, q.b2);
-            const bool in = w > theta || (w == theta && tied < quota);
-            tied += w == theta;
-            run += in ? w : 0;
-            if (in && run > target) {
-                p.token[r] = i;
-                if (p.kept) p.kept[r] = static_cast<int32_t>(above_n + quota);
-                if (p.prob) p.prob[r] = static_cast<int32_t>(((static_cast<uint64_t>(w) << 30) + (mass >> 1)) / mass);
-                break;
+    // this warp's part of row r to shared memory, masked behind the row's end
+    auto copy = [&](int r) {
+        if (r < p.n_rows) {
+            const int at = base - lane * 4 * ch;  // the warp's first logit
+            const int32_t* row = p.logits + r * p.ld + at;
+            int owner = lane / ch, k = lane - owner * ch;
+            const int step_o = 32 / ch, step_k = 32 - step_o * ch;
+#pragma unroll 4
+            for (int c = lane; c < 32 * ch; c += 32) {
+                const int place = k + shift_of(owner);
+                uint4* dst = warp_buf + owner * ch + (place >= ch ? place - ch : place);
+                const int left = p.vocab - at - 4 * c;
+                if (aligned && left >= 4) cp_async16(dst, row + 4 * c);
+                else
+                    for (int j = 0; j < 4; ++j) {
+                        if (j < left) cp_async4(reinterpret_cast<uint32_t*>(dst) + j, row + 4 * c + j);
+                        else reinterpret_cast<int32_t*>(dst)[j] = SAMPLE_MASKED;
+                    }
+                owner += step_o;
+                k += step_k;
+                if (k >= ch) {
+                    k -= ch;
+                    ++owner;
+                }
             }
         }
+        cp_async_commit();
+    };
+    // sums over the block's threads, in every thread
+    auto total = [&](uint64_t& m, uint32_t& n) {
+        turn ^= 1;
+        m = warp_sum47(m);
+        n = __reduce_add_sync(~0u, n);
+        if (lane == 0) {
+            sh.warp_mass[turn][warp] = m;
+            sh.warp_n[turn][warp] = n;
+        }
+        __syncthreads();
+        m = warp_sum47(sh.warp_mass[turn][lane]);
+        n = __reduce_add_sync(~0u, sh.warp_n[turn][lane]);
+    };
+    // ... and over the cluster's
+    auto total_cluster = [&](uint64_t& m, uint32_t& n) {
+        total(m, n);
+        if (cs > 1) {
+            if (tid == 0) {
+                sh.block_mass[turn] = m;
+                sh.block_n[turn] = n;
+            }
+            cluster_barrier();
+            m = warp_sum47(lane < cs ? static_cast<uint64_t>(ld_remote64(remote_smem(&sh.block_mass[turn], lane))) : 0);
+            n = __reduce_add_sync(~0u, lane < cs ? static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], lane))) : 0);
+        }
+    };
+    // sums over the threads before this one (and, with `blocks`, the blocks before this one)
+    auto before = [&](uint64_t m, uint32_t n, bool blocks, uint64_t& M, uint32_t& N) {
+        uint64_t sm = m;
+        uint32_t sn = n;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const uint64_t x = __shfl_up_sync(~0u, sm, o);
+            const uint32_t y = __shfl_up_sync(~0u, sn, o);
+            if (lane >= o) {
+                sm += x;
+                sn += y;
+            }
+        }
+        turn ^= 1;
+        if (lane == 31) {
+            sh.warp_mass[turn][warp] = sm;
+            sh.warp_n[turn][warp] = sn;
+        }
+        __syncthreads();
+        const uint64_t pm = sh.warp_mass[turn][lane];
+        const uint32_t pn = sh.warp_n[turn][lane];
+        M = sm - m + warp_sum47(lane < warp ? pm : 0);
+        N = sn - n + __reduce_add_sync(~0u, lane < warp ? pn : 0);
+        if (blocks) {
+            const uint64_t bm = warp_sum47(pm);
+            const uint32_t bn = __reduce_add_sync(~0u, pn);
+            if (tid == 0) {
+                sh.block_mass[turn] = bm;
+                sh.block_n[turn] = bn;
+            }
+            cluster_barrier();
+            M += warp_sum47(lane < rank ? static_cast<uint64_t>(ld_remote64(remote_smem(&sh.block_mass[turn], lane))) : 0);
+            N += __reduce_add_sync(~0u, lane < rank ? static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], lane))) : 0);
+        }
+    };
+
+    copy(blockIdx.x / cs);
+    for (int r = blockIdx.x / cs; r < p.n_rows; r += step) {
+        const SampleRow q = sample_row(p, r);
+        const uint32_t u = p.u[r];
+        cp_async_wait<0>();
+        __syncwarp();
+        int32_t mx = SAMPLE_MASKED;
+        each([&](int, uint4* x) {
+            const int4 v = *reinterpret_cast<int4*>(x);
+            mx = max(mx, max(max(v.x, v.y), max(v.z, v.w)));
+        });
+        const int32_t own_max = mx;
+        turn ^= 1;
+        mx = __reduce_max_sync(~0u, mx);
+        if (lane == 0) sh.warp_max[turn][warp] = mx;
+        __syncthreads();
+        mx = __reduce_max_sync(~0u, sh.warp_max[turn][lane]);
+        if (cs > 1) {
+            if (tid == 0) sh.block_max[turn] = mx;
+            cluster_barrier();
+            mx = __reduce_max_sync(~0u, lane < cs ? ld_remote32(remote_smem(&sh.block_max[turn], lane)) : SAMPLE_MASKED);
+        }
+        if (!q.ok || mx == SAMPLE_MASKED) {  // (the whole cluster agrees)
+            if (tid == 0 && rank == 0) {
+                if (!q.ok) atomicCAS(p.err, 0, ERR_SAMPLE_PARAM);
+                p.token[r] = -1;
+                if (p.kept) p.kept[r] = 0;
+                if (p.prob) p.prob[r] = 0;
+            }
+            copy(r + step);
+            continue;
+        }
+        // Weights.  min-p first, whose cut is known: weights below it go.  (All three keep prefixes of one order.)
+        uint64_t mass = 0;
+        uint32_t n = 0, some = 0;
+        const uint32_t least = max(static_cast<uint32_t>(q.mp) << 14, 1u);
+        auto weigh_all = [&](auto with_min) {
+            each([&](int k, uint4* x) {
+                uint4 v = *x;
+                auto weigh = [&](uint32_t l) {
+                    const uint32_t w = sample_weight(static_cast<int32_t>(l), mx, q.b2);
+                    if (!decltype(with_min)::value) {
+                        n += w != 0;
+                        return w;
+                    }
+                    n += w >= least;
+                    return w >= least ? w : 0;
+                };
+                v = make_uint4(weigh(v.x), weigh(v.y), weigh(v.z), weigh(v.w));
+                *x = v;
+                mass += v.x + v.y;  // (at most 2^31)
+                mass += v.z + v.w;
+                if (k == ch >> 1) some = v.x;
+            });
+        };
+        if (q.mp) weigh_all(std::true_type{});
+        else weigh_all(std::false_type{});
+        total_cluster(mass, n);
+
+        // theta, the mass and the number of the weights above it, and how many equal to it are kept
+        uint32_t theta = 0, above_n = n;
+        uint64_t above = mass, quota = 0;
+        uint32_t list_n = 0;
+        bool listed = false;  // the list holds all that is kept
+        const uint32_t* lw = sh.w;
+        const uint32_t* li = sh.i;
+#pragma unroll 1
+        for (int stage = 0; stage < 2; ++stage) {
+            const bool by_count = stage == 0;  // top-k, then top-p
+            uint64_t goal;
+            if (by_count) {
+                if (q.k == 0 || static_cast<uint32_t>(q.k) >= n) continue;
+                goal = q.k;
+            } else {
+                if (q.p >= 65536) continue;
+                goal = sample_goal(mass, q.p);
+                if (above < goal) {  // (within the ties that top-k kept)
+                    quota = (goal - above + theta - 1) / theta;
+                    mass = above + quota * theta;
+                    continue;
+                }
+            }
+            // The largest theta whose weights >= theta number or weigh `goal` lies in [lo, hi), where c weights (at most)
+            // are; hi_mass and hi_n are above.  Weights up to (above - goal) / vocab, all together, are not missed.
+            uint32_t lo = theta + 1, hi = SAMPLE_TOP, hi_n = 0, c = above_n;
+            uint64_t hi_mass = 0;
+            if (!by_count) lo = max(lo, static_cast<uint32_t>((above - goal) / static_cast<uint32_t>(p.vocab)) + 1);
+            auto middle = [&]() {
+                if (hi > 4 * lo) return 1u << ((63 - __clz(lo) - __clz(hi)) / 2);  // (between: their lengths differ by two)
+                return lo + (hi - lo) / 2;
+            };
+            // narrows the window to [mid, hi), with mass m and x weights, or to [lo, mid)
+            auto narrow = [&](uint32_t mid, uint64_t m, uint32_t x) {
+                if ((by_count ? hi_n + x : hi_mass + m) >= goal) {
+                    lo = mid;
+                    c = x;
+                } else {
+                    hi = mid;
+                    hi_mass += m;
+                    hi_n += x;
+                    c -= x;
+                }
+            };
+            if (!listed) {
+                const uint32_t room = cs > 1 ? SAMPLE_LIST / 2 : SAMPLE_LIST;
+                // Where to look first.  For a count: the greatest of 1024 thresholds that `goal` threads' largest weights
+                // reach, which as many weights then do.  For a mass: a sample of one weight per thread tells where the
+                // mass that may be missed, less and more a quarter, is expected to lie below.  (Not worth it where a pass
+                // is short: one row of 49152 on four blocks takes 20 us without and 25 with.)
+                uint32_t guess_lo = 0, guess_hi = 0;
+                if (c > room && ch >= SAMPLE_GUESS_CHUNKS && (!by_count || goal <= SAMPLE_THREADS / 2)) {
+                    const uint32_t top = sample_weight(own_max, mx, q.b2);
+                    sh.w[tid] = by_count ? (top >= least ? top : 0) : some;
+                    __syncthreads();
+                    uint32_t at[2] = {0, 0}, unit[2] = {1, 1};
+                    const uint64_t scale = 4 * ch * cs, want = by_count ? goal : above - goal;
+#pragma unroll 1
+                    for (int round = 0; round < 2; ++round) {
+                        // warp b's threshold: the octave 2^b, then its 32nd parts
+                        const uint32_t th0 = round == 0 ? 1u << warp : at[0] + warp * unit[0];
+                        const uint32_t th1 = round == 0 ? 1u << warp : at[1] + warp * unit[1];
+                        uint64_t f0 = 0, f1 = 0;
+#pragma unroll 4
+                        for (int i = lane; i < SAMPLE_THREADS; i += 32) {
+                            const uint32_t w = sh.w[i];
+                            if (by_count) f0 += w >= th0;
+                            else {
+                                f0 += w < th0 ? w : 0;
+                                f1 += w < th1 ? w : 0;
+                            }
+                        }
+                        f0 = warp_sum47(f0);
+                        f1 = warp_sum47(f1);
+                        turn ^= 1;
+                        if (lane == 0) {
+                            sh.warp_mass[turn][warp] = f0;
+                            reinterpret_cast<uint64_t*>(sh.few)[warp] = f1;
+                        }
+                        __syncthreads();
+                        f0 = sh.warp_mass[turn][lane];
+                        f1 = reinterpret_cast<const uint64_t*>(sh.few)[lane];
+                        const bool in0 = by_count ? f0 >= want : 4 * scale * f0 <= 3 * want;  // (true up to some threshold)
+                        const bool in1 = 4 * scale * f1 <= 5 * want;
+                        const int b0 = 31 - __clz(__ballot_sync(~0u, in0)), b1 = 31 - __clz(__ballot_sync(~0u, in1));
+                        at[0] = round == 0 ? 1u << max(b0, 0) : at[0] + max(b0, 0) * unit[0];
+                        at[1] = round == 0 ? 1u << max(b1, 0) : at[1] + max(b1, 0) * unit[1];
+                        unit[0] = max(at[0] >> 5, 1u);
+                        unit[1] = max(at[1] >> 5, 1u);
+                        if (by_count && b0 < 0) at[0] = 0;  // (fewer threads than that have any weight)
+                        __syncthreads();
+                    }
+                    guess_lo = at[0];
+                    guess_hi = by_count ? 0 : at[1] + unit[1];
+                    if (cs > 1) {  // the first block's guess is the cluster's
+                        turn ^= 1;
+                        if (tid == 0) {
+                            sh.block_n[turn] = guess_lo;
+                            sh.block_mass[turn] = guess_hi;
+                        }
+                        cluster_barrier();
+                        guess_lo = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], 0)));
+                        guess_hi = static_cast<uint32_t>(ld_remote64(remote_smem(&sh.block_mass[turn], 0)));
+                    }
+                }
+                auto pass = [&](uint32_t mid) {
+                    uint64_t m = 0;
+                    uint32_t x = 0;
+                    each([&](int, uint4* at) {
+                        const uint4 v = *at;
+                        uint32_t y = v.x >= mid ? v.x : 0, z = v.z >= mid ? v.z : 0;
+                        x += (v.x >= mid) + (v.y >= mid) + (v.z >= mid) + (v.w >= mid);
+                        y += v.y >= mid ? v.y : 0;
+                        z += v.w >= mid ? v.w : 0;
+                        m += y;
+                        m += z;
+                    });
+                    total_cluster(m, x);
+                    narrow(mid, m - hi_mass, x - hi_n);
+                };
+                for (int k = 0; c > room && hi - lo > 1; ++k) {
+                    const uint32_t guess = k == 0 ? guess_lo : k == 1 ? guess_hi : 0;
+                    pass(guess > lo && guess < hi ? guess : middle());
+                }
+                if (hi - lo > 1) {
+                    // the window's weights and indices, in index order
+                    uint32_t x = 0;
+                    each([&](int, uint4* at) {
+                        const uint4 v = *at;
+                        x += (v.x - lo < hi - lo) + (v.y - lo < hi - lo) + (v.z - lo < hi - lo) + (v.w - lo < hi - lo);
+                    });
+                    uint64_t none;
+                    uint32_t at;
+                    before(0, x, false, none, at);
+                    if (x)
+                        each([&](int k, uint4* from) {
+                            const uint4 v = *from;
+                            auto put = [&](uint32_t w, int j) {
+                                if (w - lo < hi - lo) {
+                                    sh.w[at] = w;
+                                    sh.i[at] = base + 4 * k + j;
+                                    ++at;
+                                }
+                            };
+                            put(v.x, 0);
+                            put(v.y, 1);
+                            put(v.z, 2);
+                            put(v.w, 3);
+                        });
+                    if (cs > 1) {
+                        if (tid == SAMPLE_THREADS - 1) sh.block_n[turn] = at;
+                        cluster_barrier();
+                        uint32_t to = 0;
+                        for (int b = 0; b < cs; ++b) {
+                            const uint32_t have = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], b)));
+                            for (uint32_t i = tid; i < have; i += SAMPLE_THREADS) {
+                                sh.w[SAMPLE_LIST / 2 + to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.w[i], b)));
+                                sh.i[SAMPLE_LIST / 2 + to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.i[i], b)));
+                            }
+                            to += have;
+                        }
+                        list_n = to;
+                        lw = sh.w + SAMPLE_LIST / 2;
+                        li = sh.i + SAMPLE_LIST / 2;
+                        cluster_barrier();
+                    } else {
+                        if (tid == SAMPLE_THREADS - 1) sh.few_n = at;
+                        __syncthreads();
+                        list_n = sh.few_n;
+                    }
+                    c = list_n;
+                    listed = hi == SAMPLE_TOP;
+                }
+            }
+            while (c > SAMPLE_FEW && hi - lo > 1) {
+                const uint32_t mid = middle();
+                uint64_t m = 0;
+                uint32_t x = 0;
+                for (uint32_t i = tid; i < list_n; i += SAMPLE_THREADS) {
+                    const uint32_t w = lw[i];
+                    if (w - mid < hi - mid) {
+                        m += w;
+                        ++x;
+                    }
+                }
+                total(m, x);
+                narrow(mid, m, x);
+            }
+            if (hi - lo > 1) {
+                __syncthreads();
+                if (tid == 0) sh.few_n = 0;
+                __syncthreads();
+                for (uint32_t i = tid; i < list_n; i += SAMPLE_THREADS) {
+                    const uint32_t w = lw[i];
+                    if (w - lo < hi - lo) sh.few[atomicAdd(&sh.few_n, 1u)] = w;
+                }
+                __syncthreads();
+                const uint32_t few_n = sh.few_n;
+                // warp b: candidates b, b + 32, ...
+                for (uint32_t j = warp; j < few_n; j += SAMPLE_WARPS) {
+                    const uint32_t mine = sh.few[j];
+                    uint64_t m = 0;  // of those above mine
+                    uint32_t x = 0, same = 0;
+                    for (uint32_t i = lane; i < few_n; i += 32) {
+                        const uint32_t w = sh.few[i];
+                        if (w > mine) {
+                            m += w;
+                            ++x;
+                        }
+                        same += w == mine;
+                    }
+                    m = warp_sum47(m) + hi_mass;
+                    x = __reduce_add_sync(~0u, x) + hi_n;
+                    same = __reduce_add_sync(~0u, same);
+                    // (warps of equal weights write equal words)
+                    if (lane == 0 && (by_count ? x : m) < goal &&
+                        (by_count ? x + same : m + static_cast<uint64_t>(same) * mine) >= goal) {
+                        sh.theta = mine;
+                        sh.above = m;
+                        sh.above_n = x;
+                    }
+                }
+                __syncthreads();
+                theta = sh.theta;
+                above = sh.above;
+                above_n = sh.above_n;
+            } else {
+                theta = lo;
+                above = hi_mass;
+                above_n = hi_n;
+            }
+            quota = by_count ? goal - above_n : (goal - above + theta - 1) / theta;
+            mass = above + quota * theta;
+        }
+        const uint64_t target = sample_target(mass, u);
+
+        // The draw: kept mass and ties of each thread's part of the list or of the row, in index order.
+        uint64_t m = 0;
+        uint32_t t = 0;
+        uint32_t i0 = 0, i1 = 0;
+        if (listed) {
+            const uint32_t per = (list_n + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
+            i0 = min(tid * per, list_n);
+            i1 = min(i0 + per, list_n);
+            for (uint32_t i = i0; i < i1; ++i) {
+                const uint32_t w = lw[i];
+                m += w > theta ? w : 0;
+                t += w == theta;
+            }
+        } else {
+            each([&](int, uint4* at) {
+                const uint4 v = *at;
+                uint32_t y = v.x > theta ? v.x : 0, z = v.z > theta ? v.z : 0;
+                t += (v.x == theta) + (v.y == theta) + (v.z == theta) + (v.w == theta);
+                y += v.y > theta ? v.y : 0;
+                z += v.w > theta ? v.w : 0;
+                m += y;
+                m += z;
+            });
+        }
+        uint64_t cur;
+        uint32_t ties;
+        before(m, t, cs > 1 && !listed, cur, ties);
+        uint64_t used = ties;
+        cur += theta * min(used, quota);
+        if (cur <= target && target < cur + m + theta * min(static_cast<uint64_t>(t), quota - min(quota, used)) && (!listed || rank == 0)) {
+            // one thread; its kept weights up to the target
+            uint32_t won = 0;
+            int at = -1;
+            auto look = [&](uint32_t w, int i) {
+                const bool in = w > theta || (w == theta && used < quota);
+                used += w == theta;
+                if (in && cur <= target) {  // (the last one that starts at or before the target)
+                    won = w;
+                    at = i;
+                    cur += w;
+                }
+            };
+            if (listed)
+                for (uint32_t i = i0; i < i1; ++i) look(lw[i], static_cast<int>(li[i]));
+            else
+                each([&](int k, uint4* from) {
+                    const uint4 v = *from;
+                    look(v.x, base + 4 * k);
+                    look(v.y, base + 4 * k + 1);
+                    look(v.z, base + 4 * k + 2);
+                    look(v.w, base + 4 * k + 3);
+                });
+            p.token[r] = at;
+            if (p.kept) p.kept[r] = static_cast<int32_t>(above_n + quota);
+            if (p.prob) p.prob[r] = static_cast<int32_t>(((static_cast<uint64_t>(won) << 30) + (mass >> 1)) / mass);
+        }
+        __syncwarp();
+        copy(r + step);   // (the warp has read its part of the row)
+        __syncthreads();  // the list has been read
     }
+    cp_async_wait<0>();
+    if (cs > 1) cluster_barrier();  // no block leaves while its words are read
 }
 
 }  // namespace eii
