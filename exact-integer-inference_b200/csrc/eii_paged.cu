@@ -59,12 +59,22 @@ int check_ld(const char* name, int64_t ld, int64_t least) {
 }
 
 template <int HD, int BITS>
-int launch_append(const AppendParams& ap, int in_bits, cudaStream_t st) {
-    const int64_t warps = static_cast<int64_t>(ap.n_rows) * ((ap.q ? ap.g.n_heads : 0) + 2 * ap.g.n_kv);
-    const int64_t blocks = (warps + 7) / 8;
+int launch_append(const AppendParams& ap, int in_bits, int num_sms, cudaStream_t st) {
+    // one warp per row, more while that leaves the SMs short of warps and there are heads to share
+    constexpr int at_once = AppendLanes<HD>::HEADS;
+    const int steps = (ap.q ? (ap.g.n_heads + at_once - 1) / at_once : 0) + 2 * ((ap.g.n_kv + at_once - 1) / at_once);
+    int wpr = 1;
+    while (wpr < steps && static_cast<int64_t>(ap.n_rows) * wpr < 32 * num_sms) ++wpr;
+    const int64_t blocks = (static_cast<int64_t>(ap.n_rows) * wpr + 7) / 8;
     if (blocks > INT32_MAX) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
-    if (in_bits == 16) k_paged_append<HD, BITS, int16_t><<<(unsigned)blocks, 256, 0, st>>>(ap);
-    else k_paged_append<HD, BITS, int32_t><<<(unsigned)blocks, 256, 0, st>>>(ap);
+    const int64_t e = in_bits / 8;
+    const uintptr_t in = reinterpret_cast<uintptr_t>(ap.q) | reinterpret_cast<uintptr_t>(ap.k) | reinterpret_cast<uintptr_t>(ap.v) |
+                         static_cast<uintptr_t>((ap.q ? ap.ldq : 0) * e | ap.ldk * e | ap.ldv * e);
+    const int vec_in = (in & (4 * e - 1)) == 0;
+    const int vec_out = (((reinterpret_cast<uintptr_t>(ap.q_out) | static_cast<uintptr_t>(ap.ldqo * 2)) & 7) == 0) |
+                        ((reinterpret_cast<uintptr_t>(ap.kv_out) & 15) == 0) << 1;
+    if (in_bits == 16) k_paged_append<HD, BITS, int16_t><<<(unsigned)blocks, 256, 0, st>>>(ap, wpr, vec_in, vec_out);
+    else k_paged_append<HD, BITS, int32_t><<<(unsigned)blocks, 256, 0, st>>>(ap, wpr, vec_in, vec_out);
     CK(cudaGetLastError());
     return EII_OK;
 }
@@ -276,8 +286,9 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
     ap.rope_c = p->rope_c; ap.rope_s = p->rope_s; ap.n_pos = p->n_pos; ap.shift_q = shift_q; ap.shift_k = shift_k;
     ap.q_out = q_out; ap.ldqo = ldqo; ap.kv_out = kv_out;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p->hd == 64) return p->bits == 4 ? launch_append<64, 4>(ap, in_bits, st) : launch_append<64, 16>(ap, in_bits, st);
-    return p->bits == 4 ? launch_append<128, 4>(ap, in_bits, st) : launch_append<128, 16>(ap, in_bits, st);
+    if (p->hd == 64) return p->bits == 4 ? launch_append<64, 4>(ap, in_bits, p->num_sms, st)
+                                          : launch_append<64, 16>(ap, in_bits, p->num_sms, st);
+    return p->bits == 4 ? launch_append<128, 4>(ap, in_bits, p->num_sms, st) : launch_append<128, 16>(ap, in_bits, p->num_sms, st);
 }
 
 int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, int64_t ldq, int n_rows,

@@ -65,93 +65,207 @@ struct AppendParams {
     int32_t* kv_out;
 };
 
-// Writes one lane's HD / 32 values of a cached row: x[i] is dimension lane + 32 i.
-template <int HD, int BITS>
-__device__ __forceinline__ void store_row(const PagedGeom& g, uint8_t* slab, int slot, int lane, int32_t (&x)[HD / 32]) {
-    if constexpr (BITS == 16) {
-        int16_t* row = reinterpret_cast<int16_t*>(slab) + slot * HD;
+// SAT16(x >> shift) with the rounding half already added to x, |x| >> `fits` below 2^31.  From a shift of
+// `fits` to 31 the low word is the answer, one above is taken in two steps; below `fits` (at most 16) x is
+// clamped to 2^30 first, which changes only values that saturate.
+struct Requant16 {
+    int down, rest;
+    bool clamp;
+    int64_t half;
+    __device__ Requant16(int shift, int fits)
+        : down(min(shift, 32)), rest(max(shift - 32, 0)), clamp(shift < fits), half(int64_t(1) << (shift - 1)) {}
+    __device__ __forceinline__ int32_t operator()(int64_t x) const {
+        if (clamp) x = max(min(x, (int64_t(1) << 30) - 1), -(int64_t(1) << 30));
+        const int32_t s = static_cast<int32_t>(__funnelshift_rc(static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), down)) >> rest;
+        return max(min(s, 32767), -32768);
+    }
+};
+
+// The lanes of a head: each has dimensions 4 l .. 4 l + 3 and the same of the other half.
+template <int HD>
+struct AppendLanes {
+    static constexpr int LANES = HD / 8, HEADS = 32 / LANES;  // of one warp
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* src, bool vec, int32_t (&x)[4]) {
+    if (!vec) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) row[lane + 32 * i] = static_cast<int16_t>(x[i]);
+        for (int i = 0; i < 4; ++i) x[i] = src[i];
+    } else if constexpr (sizeof(T) == 4) {
+        const int4 w = *reinterpret_cast<const int4*>(src);
+        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
     } else {
-        uint8_t* row = slab + slot * (HD / 2);
-        uint32_t* scale = reinterpret_cast<uint32_t*>(slab + (HD / 2 << g.page_shift)) + slot * (HD / 64);
-#pragma unroll
-        for (int a = 0; a < HD / 64; ++a) {
-            const int32_t lo = __reduce_min_sync(~0u, min(x[2 * a], x[2 * a + 1]));
-            const int32_t hi = __reduce_max_sync(~0u, max(x[2 * a], x[2 * a + 1]));
-            const uint32_t m = max(1u, static_cast<uint32_t>(hi - lo + 14) / 15u);
-            // n = floor((2 (x - z) + m) / (2 m)) <= 15: (hi - z) / m <= 15
-            const uint32_t n0 = (2u * static_cast<uint32_t>(x[2 * a] - lo) + m) / (2u * m);
-            const uint32_t n1 = (2u * static_cast<uint32_t>(x[2 * a + 1] - lo) + m) / (2u * m);
-            row[32 * a + lane] = static_cast<uint8_t>(n0 | (n1 << 4));
-            if (lane == 0) scale[a] = m | (static_cast<uint32_t>(lo) << 16);
-            x[2 * a] = lo + static_cast<int32_t>(m * n0);
-            x[2 * a + 1] = lo + static_cast<int32_t>(m * n1);
-        }
+        const int2 w = *reinterpret_cast<const int2*>(src);
+        x[0] = static_cast<int16_t>(w.x); x[1] = w.x >> 16; x[2] = static_cast<int16_t>(w.y); x[3] = w.y >> 16;
     }
 }
 
-// One warp per (row, head of q | k | v).
+// Nibbles of a group's values x (each lane's four of a or b) for a span of `lanes` lanes that share the group;
+// x becomes what the nibbles stand for.  floor(n / d) for n < 2^18, d = 2 m <= 2^13.1 is umulhi(n, floor((2^32 -
+// 1) / d) + 1): the reciprocal's error adds less than 2^-14 to a quotient whose fraction is a multiple of 1 / d.
+template <int LANES, int N>
+__device__ __forceinline__ uint32_t quantise4(int32_t (&x)[N], uint32_t (&nib)[N]) {
+    int32_t lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+        lo = min(lo, x[i]);
+        hi = max(hi, x[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) {
+        lo = min(lo, __shfl_xor_sync(~0u, lo, o));
+        hi = max(hi, __shfl_xor_sync(~0u, hi, o));
+    }
+    const uint32_t m = max(1u, static_cast<uint32_t>(hi - lo + 14) / 15u), rcp = 0xFFFFFFFFu / (2 * m) + 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        nib[i] = __umulhi(2 * static_cast<uint32_t>(x[i] - lo) + m, rcp);
+        x[i] = lo + static_cast<int32_t>(m * nib[i]);
+    }
+    return m | (static_cast<uint32_t>(lo) << 16);
+}
+
+// `wpr` warps per row take turns at its steps: four (two) heads of q, then of k, then of v, HD / 8 lanes each; the
+// row's position, page and each lane's four cosines and sines stay in registers.  16-byte loads of int32
+// inputs, 8-byte ones of int16, element by element where alignment does not allow them.
 template <int HD, int BITS, typename T>
-__global__ void __launch_bounds__(256) k_paged_append(const AppendParams p) {
-    constexpr int N = HD / 32;
+__global__ void __launch_bounds__(256) k_paged_append(const AppendParams p, const int wpr, const int vec_in, const int vec_out) {
+    constexpr int LANES = AppendLanes<HD>::LANES, HEADS = AppendLanes<HD>::HEADS, HALF = HD / 2;
     const PagedGeom& g = p.g;
-    const int lane = threadIdx.x & 31;
-    const int nq = p.q ? g.n_heads : 0, heads = nq + 2 * g.n_kv;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (item >= static_cast<int64_t>(p.n_rows) * heads) return;
-    const int r = static_cast<int>(item / heads), h = static_cast<int>(item % heads);
+    const int lane = threadIdx.x & 31, l = lane % LANES, sub = lane / LANES;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int r = static_cast<int>(index / wpr);
+    if (r >= p.n_rows) return;
     const int seq = p.seq ? p.seq[r] : r, pos = p.pos[r];
     if (seq < 0 || pos < 0) return;  // a padding row
     if (seq >= g.n_seq || pos >= p.n_pos || (pos >> g.page_shift) >= g.ld_table) {
         if (lane == 0) atomicCAS(g.err, 0, seq >= g.n_seq ? ERR_PAGED_SEQ : ERR_PAGED_POS);
         return;
     }
-    const bool is_q = h < nq, is_v = h >= nq + g.n_kv;
-    const int head = is_q ? h : is_v ? h - nq - g.n_kv : h - nq;
-    const T* src = is_q ? static_cast<const T*>(p.q) + r * p.ldq
-                        : is_v ? static_cast<const T*>(p.v) + r * p.ldv : static_cast<const T*>(p.k) + r * p.ldk;
-    int page_id = 0;
-    if (!is_q) {
-        page_id = g.table[seq * g.ld_table + (pos >> g.page_shift)];
-        if (page_id < 0 || page_id >= g.n_pages) {
-            if (lane == 0) atomicCAS(g.err, 0, ERR_PAGED_PAGE);
-            return;
-        }
-    }
-    int32_t x[N];
-    bool bad = false;
+    const int page_id = g.table[seq * g.ld_table + (pos >> g.page_shift)];
+    const int4 c4 = *reinterpret_cast<const int4*>(p.rope_c + static_cast<int64_t>(pos) * HALF + 4 * l);
+    const int4 s4 = *reinterpret_cast<const int4*>(p.rope_s + static_cast<int64_t>(pos) * HALF + 4 * l);
+    const int32_t cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+    const int steps_q = p.q ? (g.n_heads + HEADS - 1) / HEADS : 0, steps_kv = (g.n_kv + HEADS - 1) / HEADS;
+
+    // this lane's eight values of a head; true when all of the head's lie in the int16 range
+    auto load8 = [&](const T* src, int32_t (&x)[8]) {
+        int32_t a[4], b[4];
+        load4(src + 4 * l, vec_in, a);
+        load4(src + HALF + 4 * l, vec_in, b);
+        uint32_t over = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        x[i] = src[head * HD + lane + 32 * i];
-        bad |= x[i] != static_cast<int16_t>(x[i]);
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+            over |= static_cast<uint32_t>(a[i] + 32768) | static_cast<uint32_t>(b[i] + 32768);
+        }
+        if constexpr (sizeof(T) == 2) return true;
+        const uint32_t mine = ((1ull << LANES) - 1) << (sub * LANES);
+        if ((__ballot_sync(~0u, over >> 16 != 0) & mine) == 0) return true;
+        if (l == 0) atomicCAS(g.err, 0, ERR_PAGED_INPUT);
+        return false;
+    };
+    // |sum| <= 2^46: a shift of 16 to 31 leaves 32 bits, which the caller saturates
+    auto rotate8 = [&](int32_t (&x)[8], int shift) {
+        const Requant16 down(shift, 16);
+        const bool plain = shift >= 16 && shift <= 31;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t u = static_cast<int64_t>(x[i]) * cv[i] + down.half - static_cast<int64_t>(x[4 + i]) * sv[i];
+            const int64_t w = static_cast<int64_t>(x[4 + i]) * cv[i] + down.half + static_cast<int64_t>(x[i]) * sv[i];
+            if (plain) {
+                x[i] = static_cast<int32_t>(__funnelshift_r(static_cast<uint32_t>(u), static_cast<uint32_t>(u >> 32), shift));
+                x[4 + i] = static_cast<int32_t>(__funnelshift_r(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), shift));
+            } else {
+                x[i] = down(u);
+                x[4 + i] = down(w);
+            }
+        }
+    };
+    auto store8 = [&](int16_t* o, const int32_t (&x)[8], bool vec) {
+        const uint2 a = make_uint2(pack_sat_s16(x[1], x[0]), pack_sat_s16(x[3], x[2]));
+        const uint2 b = make_uint2(pack_sat_s16(x[5], x[4]), pack_sat_s16(x[7], x[6]));
+        o += 4 * l;
+        if (vec) {
+            *reinterpret_cast<uint2*>(o) = a;
+            *reinterpret_cast<uint2*>(o + HALF) = b;
+        } else {
+            o[0] = a.x; o[1] = a.x >> 16; o[2] = a.y; o[3] = a.y >> 16;
+            o[HALF] = b.x; o[HALF + 1] = b.x >> 16; o[HALF + 2] = b.y; o[HALF + 3] = b.y >> 16;
+        }
+    };
+
+    int step = static_cast<int>(index % wpr);
+#pragma unroll 2
+    for (; step < steps_q; step += wpr) {
+        const int head = step * HEADS + sub, from = min(head, g.n_heads - 1);  // (lanes behind the last head repeat it)
+        int32_t x[8];
+        const bool good = load8(static_cast<const T*>(p.q) + r * p.ldq + from * HD, x);
+        rotate8(x, p.shift_q);
+        if (good && head < g.n_heads) store8(p.q_out + r * p.ldqo + head * HD, x, vec_out & 1);
     }
-    if (__any_sync(~0u, bad)) {
-        if (lane == 0) atomicCAS(g.err, 0, ERR_PAGED_INPUT);
+    if (step >= steps_q + 2 * steps_kv) return;
+    if (page_id < 0 || page_id >= g.n_pages) {
+        if (lane == 0) atomicCAS(g.err, 0, ERR_PAGED_PAGE);
         return;
     }
-    if (!is_v) {
-        const int shift = is_q ? p.shift_q : p.shift_k;
-        const int64_t half = HD / 2;
+    const int slot = pos & ((1 << g.page_shift) - 1);
+#pragma unroll 1
+    for (; step < steps_q + 2 * steps_kv; step += wpr) {
+        const bool is_v = step >= steps_q + steps_kv;
+        const int head = (step - steps_q - (is_v ? steps_kv : 0)) * HEADS + sub, from = min(head, g.n_kv - 1);
+        int32_t x[8];
+        bool good = load8((is_v ? static_cast<const T*>(p.v) + r * p.ldv : static_cast<const T*>(p.k) + r * p.ldk) + from * HD, x);
+        if (!is_v) {
+            rotate8(x, p.shift_k);
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            const int64_t c = p.rope_c[pos * half + lane + 32 * i], s = p.rope_s[pos * half + lane + 32 * i];
-            const int64_t a = x[i], b = x[i + N / 2];
-            x[i] = static_cast<int32_t>(sat64(rs64(a * c - b * s, shift), 16));
-            x[i + N / 2] = static_cast<int32_t>(sat64(rs64(b * c + a * s, shift), 16));
+            for (int i = 0; i < 8; ++i) x[i] = max(min(x[i], 32767), -32768);
         }
-    }
-    if (is_q) {
+        uint32_t bytes[HD / 64] = {}, scale[HD / 64] = {};
+        if constexpr (BITS == 4 && HD == 64) {
+            uint32_t nib[8];
+            scale[0] = quantise4<LANES>(x, nib);
+            bytes[0] = nib[0] | nib[4] << 4 | nib[1] << 8 | nib[5] << 12 | nib[2] << 16 | nib[6] << 20 | nib[3] << 24 | nib[7] << 28;
+        } else if constexpr (BITS == 4) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) p.q_out[r * p.ldqo + head * HD + lane + 32 * i] = static_cast<int16_t>(x[i]);
-        return;
-    }
-    store_row<HD, BITS>(g, (is_v ? g.v_pool : g.k_pool) + slab_offset(g, page_id, head), pos & ((1 << g.page_shift) - 1),
-                        lane, x);
-    if (p.kv_out) {
-        int32_t* o = p.kv_out + ((static_cast<int64_t>(r) * 2 + is_v) * g.n_kv + head) * HD + lane;
+            for (int a = 0; a < 2; ++a) {
+                int32_t z[4] = {x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]};
+                uint32_t n[4];
+                scale[a] = quantise4<LANES>(z, n);
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[32 * i] = x[i];
+                for (int i = 0; i < 4; ++i) x[4 * a + i] = z[i];
+                // lanes 0 .. 7 have the low nibbles, 8 .. 15 the high ones of the same bytes
+                const uint32_t own = n[0] | n[1] << 8 | n[2] << 16 | n[3] << 24, other = __shfl_xor_sync(~0u, own, 8);
+                bytes[a] = l < 8 ? own | other << 4 : other | own << 4;
+            }
+        }
+        if (!good || head >= g.n_kv) continue;
+        uint8_t* slab = (is_v ? g.v_pool : g.k_pool) + slab_offset(g, page_id, head);
+        if constexpr (BITS == 16) store8(reinterpret_cast<int16_t*>(slab) + slot * HD, x, true);
+        else {
+            uint32_t* sc = reinterpret_cast<uint32_t*>(slab + (HALF << g.page_shift)) + slot * (HD / 64);
+            // (head_dim 128: lanes 8 .. 15 hold the second group's words)
+            reinterpret_cast<uint32_t*>(slab + slot * HALF)[l] = HD == 64 || l < 8 ? bytes[0] : bytes[HD / 64 - 1];
+            if (l == 0) {
+                if constexpr (HD == 64) sc[0] = scale[0];
+                else *reinterpret_cast<uint2*>(sc) = make_uint2(scale[0], scale[1]);
+            }
+        }
+        if (p.kv_out) {
+            int32_t* o = p.kv_out + ((static_cast<int64_t>(r) * 2 + is_v) * g.n_kv + head) * HD + 4 * l;
+            if (vec_out & 2) {
+                *reinterpret_cast<int4*>(o) = make_int4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<int4*>(o + HALF) = make_int4(x[4], x[5], x[6], x[7]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = x[i];
+                    o[HALF + i] = x[4 + i];
+                }
+            }
+        }
     }
 }
 
@@ -237,22 +351,6 @@ __device__ __forceinline__ void transpose4(uint32_t x0, uint32_t x1, uint32_t x2
     r[2] = __byte_perm(t2, t3, 0x5410);
     r[3] = __byte_perm(t2, t3, 0x7632);
 }
-
-// SAT16(x >> shift) of a score with the rounding half already added.  |x| < 2^38 for every valid cache, so
-// a shift of 8 to 31 leaves 32 bits and one above is taken in two steps; below 8 x is clamped first, which
-// changes only values that saturate.
-struct ScoreShift {
-    int down, rest;
-    bool clamp;
-    int64_t half;
-    __device__ explicit ScoreShift(int shift)
-        : down(min(shift, 32)), rest(max(shift - 32, 0)), clamp(shift < 8), half(int64_t(1) << (shift - 1)) {}
-    __device__ __forceinline__ int32_t operator()(int64_t x) const {
-        if (clamp) x = max(min(x, (int64_t(1) << 30) - 1), -(int64_t(1) << 30));
-        const int32_t s = static_cast<int32_t>(__funnelshift_rc(static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), down)) >> rest;
-        return max(min(s, 32767), -32768);
-    }
-};
 
 // floor((e 2^pb + floor(z / 2)) / z) for e <= 2^30 <= z, with rcp = floor(2^61 / z) <= 2^31: e rcp / 2^(61 - pb)
 // + 1/2 lies above the quotient by at most 1 / (2 z) and below it by less than 2^30 / 2^(61 - pb) <= 2^-12, so
@@ -468,7 +566,7 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
     }
 
     // ---------------------------------------------------------------- pass 1: scores and their maximum
-    const ScoreShift shift(p.shift_s);
+    const Requant16 shift(p.shift_s, 8);  // (|scores| < 2^38 for every valid cache)
     int32_t mx[NH];
 #pragma unroll
     for (int h = 0; h < NH; ++h) mx[h] = -32768;
