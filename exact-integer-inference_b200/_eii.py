@@ -79,6 +79,11 @@ _SIGS = {
                              ctypes.c_int, ctypes.c_int, _P, ctypes.c_int64, _P], ctypes.c_int),
     "eii_paged_sync": ([_P, _P], ctypes.c_int),
     "eii_paged_close": ([_P], None),
+    "eii_paged_decoder_open": ([_P, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.POINTER(_P)], ctypes.c_int),
+    "eii_paged_decoder_step_device_async": ([_P, _P, _P, _P, ctypes.c_int, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+                                             _P, ctypes.c_int64, _P], ctypes.c_int),
+    "eii_paged_decoder_sync": ([_P, _P], ctypes.c_int),
+    "eii_paged_decoder_close": ([_P], None),
     "eii_sampler_open": ([ctypes.c_int, ctypes.POINTER(_P)], ctypes.c_int),
     "eii_sample": ([_P, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int] + [_P] * 9, ctypes.c_int),
     "eii_sampler_sync": ([_P, _P], ctypes.c_int),
@@ -469,6 +474,37 @@ class Paged:
 
     def sync(self, stream=None):
         check(lib().eii_paged_sync(self.h, stream))
+
+
+class PagedDecoder:
+    """Ragged decoding of the model on a paged cache of 16 or 4 bits (include/eii.h, eii_paged_decoder_*)."""
+
+    def __init__(self, engine, page_size, cache_bits, n_pages):
+        self.h = None
+        h = ctypes.c_void_p()
+        check(lib().eii_paged_decoder_open(engine.h, int(page_size), int(cache_bits), int(n_pages), ctypes.byref(h)))
+        self.h = h
+        self.engine = engine  # the engine must outlive the decoder
+
+    def close(self):
+        if self.h:
+            lib().eii_paged_decoder_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def step_device_async(self, ids_ptr, seq_ptr, pos_ptr, n_rows, table_ptr, ld_table, n_seq, max_len, logits_ptr=None,
+                          ld=VOCAB, stream=None):
+        """One token per row, without waiting: device-side errors surface at the next sync()."""
+        check(lib().eii_paged_decoder_step_device_async(self.h, ids_ptr, seq_ptr, pos_ptr, n_rows, table_ptr, ld_table,
+                                                        n_seq, max_len, logits_ptr, ld, stream or None))
+
+    def sync(self, stream=None):
+        check(lib().eii_paged_decoder_sync(self.h, stream or None))
 
 
 class Sampler:

@@ -27,6 +27,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -38,6 +39,7 @@
 #include "eii_tgemm.cuh"
 #include "eii_mma_probe.cuh"
 #include "eii_kernels.cuh"
+#include "eii_paged.h"
 
 using namespace eii;
 
@@ -301,6 +303,15 @@ struct eii_decoder {
     int n_seq = 0, max_T = 0, pos = 0;
     int16_t* kc = nullptr;
     int16_t* vc = nullptr;
+    std::vector<void*> mem;
+};
+
+// Pools of a paged decoder: per layer k and v, pool_bytes each.
+struct eii_paged_decoder {
+    eii_engine* e = nullptr;
+    eii_paged* cache = nullptr;
+    int64_t n_pages = 0, pool_bytes = 0;
+    uint8_t* pools = nullptr;
     std::vector<void*> mem;
 };
 
@@ -626,6 +637,15 @@ struct KvHook {
     int pos;
 };
 
+// Paged-cache hook of run_layer (eii_paged_decoder_*): every row is one token of sequence seq[r] at position
+// pos[r]; the rows are appended to the layer's pools, then attend over them.
+struct PagedHook {
+    eii_paged* cache;
+    eii_pages pages;  // this layer's
+    const int32_t *seq, *pos;
+    int max_len;
+};
+
 // Per-site trace hook of run_layer (python/intref.py:192-286 with trace): device buffers for the
 // sites the fused kernels never materialise.  The norms run a second time in their generic form
 // (U, z, int64 output), the projections and residual terms run as EPI_LINEAR GEMMs on the same
@@ -659,7 +679,7 @@ int launch_grid(eii_engine* e, int rows, int which, int l, cudaStream_t st) {
 
 // norm_done: the layer's first norm is already in h_planes (the embedding produced it).
 int run_layer(eii_engine* e, int l, int rows, int T, cudaStream_t st, const KvHook* kv = nullptr,
-              const TraceHook* trh = nullptr, bool norm_done = false) {
+              const TraceHook* trh = nullptr, bool norm_done = false, const PagedHook* pg = nullptr) {
     if (e->grid_on && !trh) TRY(launch_grid(e, rows, 0, l, st));
     LayerDev& L = e->L[l];
     const ActMaps* am;
@@ -682,12 +702,22 @@ int run_layer(eii_engine* e, int l, int rows, int T, cudaStream_t st, const KvHo
     ep.bits_q = L.q.bits; ep.bits_k = L.k.bits; ep.bits_v = L.v.bits; ep.bits_qr = L.qr.bits; ep.bits_kr = L.kr.bits;
     ep.rope_shift_q = L.rope_shift_q; ep.rope_shift_k = L.rope_shift_k; ep.fast = L.fast_qkv; ep.narrow = L.narrow_qkv;
     ep.pos0 = decode ? kv->pos : 0;
+    // (rows of a paged step are rotated by their own positions as they are appended: here T = 1, so every row gets
+    // position 0, whose rotation is the identity, and the shift of 30 takes the Q30 cosine out again)
+    if (pg) ep.rope_shift_q = ep.rope_shift_k = 30;
     TRY(launch_gemm<2, EPI_QKV>(e, am->h, L.tm_qkv, ep, st, EII_K_GEMM_QKV, &am->q, &am->k, &am->v));
 
     if (kv && !decode) {  // keep the prompt's k, v rows (T per sequence); a step's row is appended by the attention
         const size_t row = 192 * sizeof(int16_t), pitch = row * kv->max_T;
         CK(cudaMemcpy2DAsync(kv->kc, pitch, e->k, row * T, row * T, nseq, cudaMemcpyDeviceToDevice, st));
         CK(cudaMemcpy2DAsync(kv->vc, pitch, e->v, row * T, row * T, nseq, cudaMemcpyDeviceToDevice, st));
+    }
+    if (pg) {
+        ProfScope ps(e, EII_K_ATTENTION, st);
+        TRY(eii_paged_append(pg->cache, &pg->pages, e->q, D_MODEL, e->k, 192, e->v, 192, 16, rows, pg->seq, pg->pos,
+                             L.rope_shift_q, L.rope_shift_k, e->q, D_MODEL, nullptr, st));
+        TRY(paged_attention_planes(pg->cache, pg->pages, e->q, rows, pg->seq, pg->pos, pg->max_len, L.shift_s, L.shift_c,
+                                   L.c.bits, e->ctx_planes, L.Pc, L.t_o, st));
     }
     if (decode) {
         AttnDecodeParams dp{};
@@ -709,7 +739,7 @@ int run_layer(eii_engine* e, int l, int rows, int T, cudaStream_t st, const KvHo
         ap.score_out = trh->score;
         ap.prob_out = trh->prob;
     }
-    if (!decode) {
+    if (!decode && !pg) {
         ProfScope ps(e, EII_K_ATTENTION, st);
         if (T <= 128 && !e->force_cuda_core_attention && !trh) {
             // persistent: one CTA per SM (its resources allow one), each looping over (sequence, KV group) items
@@ -1584,6 +1614,107 @@ void eii_decoder_close(eii_decoder* d) {
     if (!d) return;
     cudaSetDevice(d->e->device);
     if (d->e->stream) cudaStreamSynchronize(d->e->stream);
+    free_list(d->mem);
+    delete d;
+}
+
+int eii_paged_decoder_open(eii_engine* e, int page_size, int cache_bits, int64_t n_pages, eii_paged_decoder** out) {
+    if (!out) return fail(EII_ERR_ARG, "out is null");
+    *out = nullptr;
+    if (!e) return fail(EII_ERR_ARG, "engine is null");
+    if (n_pages < 1 || n_pages > INT32_MAX) return fail(EII_ERR_ARG, "n_pages must be in [1, 2^31) (got %lld)", (long long)n_pages);
+    for (const LayerDev& L : e->L)
+        if (L.rope_shift_q < 1 || L.rope_shift_q > 62 || L.rope_shift_k < 1 || L.rope_shift_k > 62 || L.shift_s < 1 ||
+            L.shift_s > 62 || L.shift_c < -16 || L.shift_c > 62)
+            return fail(EII_ERR_FORMAT, "a layer's rope or score shift lies outside [1, 62] or its context shift outside [-16, 62]");
+    CK(cudaSetDevice(e->device));
+    eii_paged_decoder* d = nullptr;
+    try {
+        // the model's own tables; the cache's exp table is the regenerated one, so the model's has to equal it
+        std::vector<int32_t> c(ROPE_POS * 32), s(ROPE_POS * 32), x(DMAX + 1);
+        std::vector<int64_t> c64(ROPE_POS * 32), s64(ROPE_POS * 32), x64(DMAX + 1);
+        CK(cudaMemcpy(c.data(), e->rope_c, c.size() * 4, cudaMemcpyDeviceToHost));
+        CK(cudaMemcpy(s.data(), e->rope_s, s.size() * 4, cudaMemcpyDeviceToHost));
+        CK(cudaMemcpy(x.data(), e->exp_tab, x.size() * 4, cudaMemcpyDeviceToHost));
+        TRY(eii_table_exp(x64.data()));
+        for (int i = 0; i <= DMAX; ++i)
+            if (x[i] != x64[i]) return fail(EII_ERR_FORMAT, "the model's exp table differs from the regenerated one at %d", i);
+        for (int i = 0; i < ROPE_POS * 32; ++i) {
+            c64[i] = c[i];
+            s64[i] = s[i];
+        }
+        for (int i = 0; i < 32; ++i)
+            if (c[i] != 1 << 30 || s[i] != 0) return fail(EII_ERR_FORMAT, "position 0 of the model's rope tables is not the identity");
+        d = new eii_paged_decoder();
+        d->e = e;
+        d->n_pages = n_pages;
+        int rc = eii_paged_open(e->device, N_HEADS, N_KV, HEAD_DIM, page_size, cache_bits, ROPE_POS, c64.data(), s64.data(), &d->cache);
+        if (rc == EII_OK) {
+            d->pool_bytes = (eii_paged_pool_bytes(d->cache, n_pages) + 255) / 256 * 256;
+            rc = dalloc(d->mem, &d->pools, static_cast<size_t>(d->pool_bytes) * 2 * N_LAYERS);
+        }
+        if (rc != EII_OK) {
+            eii_paged_decoder_close(d);
+            return rc;
+        }
+    } catch (const std::bad_alloc&) {
+        if (d) eii_paged_decoder_close(d);
+        return fail(EII_ERR_ARG, "out of host memory");
+    }
+    *out = d;
+    return EII_OK;
+}
+
+int eii_paged_decoder_step_device_async(eii_paged_decoder* d, const int64_t* ids_dev, const int32_t* seq_dev,
+                                        const int32_t* pos_dev, int n_rows, const int32_t* table_dev, int64_t ld_table,
+                                        int n_seq, int max_len, int32_t* logits_dev, int64_t ld_logits, void* stream) {
+    if (!d) return fail(EII_ERR_ARG, "decoder is null");
+    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    if (n_rows == 0) return EII_OK;
+    if (!ids_dev || !seq_dev || !pos_dev || !table_dev) return fail(EII_ERR_ARG, "ids_dev, seq_dev, pos_dev or table_dev is null");
+    if (max_len < 1 || max_len > ROPE_POS) return fail(EII_ERR_ARG, "max_len must be in [1, %d] (got %d)", ROPE_POS, max_len);
+    if (n_seq < 1 || ld_table < 1) return fail(EII_ERR_ARG, "n_seq and ld_table must be >= 1 (got %d and %lld)", n_seq, (long long)ld_table);
+    if (logits_dev && (ld_logits < VOCAB || (ld_logits % 4) != 0 || (reinterpret_cast<uintptr_t>(logits_dev) & 15)))
+        return fail(EII_ERR_ARG, "logits_dev must be 16-byte aligned with ld >= %d, ld %% 4 == 0", VOCAB);
+    eii_engine* e = d->e;
+    CK(cudaSetDevice(e->device));
+    cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : e->stream;
+    const int cs = chunk_seqs_for(e, n_rows, 1);
+    TRY(ensure_rows(e, cs));
+    for (int r0 = 0; r0 < n_rows; r0 += cs) {
+        const int rows = n_rows - r0 < cs ? n_rows - r0 : cs;
+        bool normed = false;
+        TRY(launch_embed(e, ids_dev + r0, rows, st, &normed));
+        for (int l = 0; l < N_LAYERS; ++l) {
+            PagedHook pg{};
+            pg.cache = d->cache;
+            pg.pages.k_pool = d->pools + static_cast<size_t>(2 * l) * d->pool_bytes;
+            pg.pages.v_pool = d->pools + static_cast<size_t>(2 * l + 1) * d->pool_bytes;
+            pg.pages.n_pages = d->n_pages; pg.pages.table = table_dev; pg.pages.ld_table = ld_table; pg.pages.n_seq = n_seq;
+            pg.seq = seq_dev + r0; pg.pos = pos_dev + r0; pg.max_len = max_len;
+            TRY(run_layer(e, l, rows, 1, st, nullptr, nullptr, l == 0 && normed, &pg));
+        }
+        if (logits_dev) TRY(run_logits(e, rows, 1, logits_dev + static_cast<int64_t>(r0) * ld_logits, ld_logits, nullptr, st));
+    }
+    return EII_OK;
+}
+
+int eii_paged_decoder_sync(eii_paged_decoder* d, void* stream) {
+    if (!d) return fail(EII_ERR_ARG, "decoder is null");
+    CK(cudaSetDevice(d->e->device));
+    cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : d->e->stream;
+    const int rc = eii_paged_sync(d->cache, st), rc2 = check_device_error(d->e, st);
+    // (a bad index first: the rows it leaves undefined can make later kernels report more)
+    if (rc != EII_OK && rc2 == EII_OK) return rc;
+    if (rc != EII_OK) return fail(rc, "a sequence index, position, length or page of the step lies outside its range");
+    return rc2;
+}
+
+void eii_paged_decoder_close(eii_paged_decoder* d) {
+    if (!d) return;
+    cudaSetDevice(d->e->device);
+    if (d->e->stream) cudaStreamSynchronize(d->e->stream);
+    eii_paged_close(d->cache);
     free_list(d->mem);
     delete d;
 }

@@ -29,4 +29,13 @@ __device__ __forceinline__ uint8_t plane_byte(int64_t a, int p) {
     return static_cast<uint8_t>(static_cast<uint64_t>(a >> (8 * p)) & 0xFFu);
 }
 
+// Row-blocked planes.  // Activation byte planes read by the GEMMs through the row-blocked layout
+// [P][ceil(M/128)][K/16][128 rows][16 bytes]: byte k of row r of a plane sits at blocked_off(r, k, K),
+// so 32 consecutive rows x 16 bytes are 512 contiguous bytes (coalesced epilogue stores) and a GEMM
+// reads a 128-row x 128-byte K block as eight 2 KB runs (see map_blocked on the host).
+__host__ __device__ __forceinline__ int64_t blocked_off(int64_t r, int k, int K) {
+    return (r >> 7) * 128 * K + (k >> 4) * 2048 + (r & 127) * 16 + (k & 15);
+}
+__host__ __device__ __forceinline__ int64_t blocked_plane_stride(int64_t M, int K) { return ((M + 127) / 128) * 128 * K; }
+
 }  // namespace eii

@@ -347,16 +347,6 @@ __global__ void __launch_bounds__(256) k_embed_norm(const int64_t* __restrict__ 
     rmsnorm_pair_finish(v, row, live, M, gain, shift_out, planes, top_flip);
 }
 
-// --------------------------------------------------------------------------- row-blocked planes
-// Activation byte planes read by the GEMMs through the row-blocked layout
-// [P][ceil(M/128)][K/16][128 rows][16 bytes]: byte k of row r of a plane sits at blocked_off(r, k, K),
-// so 32 consecutive rows x 16 bytes are 512 contiguous bytes (coalesced epilogue stores) and a GEMM
-// reads a 128-row x 128-byte K block as eight 2 KB runs (see map_blocked on the host).
-__host__ __device__ __forceinline__ int64_t blocked_off(int64_t r, int k, int K) {
-    return (r >> 7) * 128 * K + (k >> 4) * 2048 + (r & 127) * 16 + (k & 15);
-}
-__host__ __device__ __forceinline__ int64_t blocked_plane_stride(int64_t M, int K) { return ((M + 127) / 128) * 128 * K; }
-
 // --------------------------------------------------------------------------- attention
 // Integer causal attention of one sequence and one KV group (3 query heads), CUDA cores.
 //   s_ij = SAT16(RS(q_i . k_j, shift_s)), j <= i; rowmax; e = E[rowmax - s] (0 beyond DMAX);

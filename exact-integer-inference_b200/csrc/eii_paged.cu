@@ -8,6 +8,7 @@
 #include "eii.h"
 #include "eii_host.h"
 #include "eii_paged.cuh"
+#include "eii_paged.h"
 
 using namespace eii;
 
@@ -291,6 +292,11 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
     return p->bits == 4 ? launch_append<128, 4>(ap, in_bits, p->num_sms, st) : launch_append<128, 16>(ap, in_bits, p->num_sms, st);
 }
 
+static int attention(eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
+    if (p->hd == 64) return p->bits == 4 ? launch_attention<64, 4>(p, ap, st) : launch_attention<64, 16>(p, ap, st);
+    return p->bits == 4 ? launch_attention<128, 4>(p, ap, st) : launch_attention<128, 16>(p, ap, st);
+}
+
 int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, int64_t ldq, int n_rows,
                         const int32_t* seq, const int32_t* len, int max_len, int shift_s, int prob_bits, int shift_c,
                         int bits_c, int32_t* ctx, int64_t ldc, void* stream) {
@@ -306,7 +312,7 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
     TRY(check_ld("ldq", ldq, (int64_t)p->n_heads * p->hd));
     TRY(check_ld("ldc", ldc, (int64_t)p->n_heads * p->hd));
     TRY(check_shift("shift_s", shift_s));
-    TRY(check_shift("shift_c", shift_c));
+    if (shift_c < -16 || shift_c > 62) return fail(EII_ERR_ARG, "shift_c must be in [-16, 62] (got %d)", shift_c);
     if (prob_bits < 16 || prob_bits > 19) return fail(EII_ERR_ARG, "prob_bits must be in [16, 19] (got %d)", prob_bits);
     if (bits_c < 2 || bits_c > 32) return fail(EII_ERR_ARG, "bits_c must be in [2, 32] (got %d)", bits_c);
     if ((reinterpret_cast<uintptr_t>(q) & 1) || (reinterpret_cast<uintptr_t>(ctx) & 3))
@@ -317,9 +323,7 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
     ap.g = geometry(p, pages);
     ap.q = q; ap.ldq = ldq; ap.n_rows = n_rows; ap.seq = seq; ap.len = len; ap.max_len = max_len;
     ap.shift_s = shift_s; ap.prob_bits = prob_bits; ap.shift_c = shift_c; ap.bits_c = bits_c; ap.ctx = ctx; ap.ldc = ldc;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p->hd == 64) return p->bits == 4 ? launch_attention<64, 4>(p, ap, st) : launch_attention<64, 16>(p, ap, st);
-    return p->bits == 4 ? launch_attention<128, 4>(p, ap, st) : launch_attention<128, 16>(p, ap, st);
+    return attention(p, ap, static_cast<cudaStream_t>(stream));
 }
 
 int eii_paged_sync(eii_paged* p, void* stream) {
@@ -342,6 +346,21 @@ int eii_paged_sync(eii_paged* p, void* stream) {
     }
     return fail(EII_ERR_DEVICE, "kernel reported error %d", code);
 }
+
+}  // extern "C"
+
+int eii::paged_attention_planes(eii_paged* p, const eii_pages& pages, const int16_t* q, int n_rows, const int32_t* seq,
+                                const int32_t* pos, int max_len, int shift_s, int shift_c, int bits_c, uint8_t* planes,
+                                int n_planes, int offset, cudaStream_t st) {
+    PagedAttnParams ap{};
+    ap.g = geometry(p, &pages);
+    ap.q = q; ap.ldq = p->n_heads * p->hd; ap.n_rows = n_rows; ap.seq = seq; ap.len = pos; ap.len_add = 1; ap.max_len = max_len;
+    ap.shift_s = shift_s; ap.prob_bits = 16; ap.shift_c = shift_c; ap.bits_c = bits_c;
+    ap.planes = planes; ap.n_planes = n_planes; ap.offset = offset;
+    return attention(p, ap, st);
+}
+
+extern "C" {
 
 void eii_paged_close(eii_paged* p) {
     if (!p) return;

@@ -278,11 +278,28 @@ struct PagedAttnParams {
     int64_t ldq;
     int n_rows;
     const int32_t *seq, *len;
+    int len_add;             // a row sees len[r] + len_add keys (len holds positions where this is 1)
     int max_len;
     int shift_s, prob_bits, shift_c, bits_c;
     int32_t* ctx;
     int64_t ldc;
+    // instead of ctx: the engine's row-blocked byte planes of n_rows rows (blocked_off), in offset binary if so
+    uint8_t* planes;
+    int n_planes, offset;
 };
+
+// Context value `col` (of all query heads) of row r from its exact sum.
+__device__ __forceinline__ void store_context(const PagedAttnParams& p, int r, int col, int64_t sum) {
+    const int64_t c = sat64(rs64(sum, p.shift_c), p.bits_c);
+    if (!p.planes) {
+        p.ctx[r * p.ldc + col] = static_cast<int32_t>(c);
+        return;
+    }
+    const int K = p.g.n_heads * p.g.hd;
+    uint8_t* at = p.planes + blocked_off(r, col, K);
+    const int64_t x = c + (p.offset ? int64_t(1) << (8 * p.n_planes - 1) : 0);
+    for (int i = 0; i < p.n_planes; ++i) at[i * blocked_plane_stride(p.n_rows, K)] = plane_byte(x, i);
+}
 
 // Geometry of the kernel below.  A tile is 32 keys of one warp.
 constexpr int PATTN_MAX_HEADS = 4;      // query heads of one item (they share a kv head)
@@ -419,7 +436,7 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
     const int ht = item % head_tiles, kv = item / head_tiles % g.n_kv, r = item / head_tiles / g.n_kv;
     const int head0 = kv * g.group + ht * NH, nh = min(NH, g.group - ht * NH);
     const int seq = p.seq ? p.seq[r] : r;
-    int len = max(p.len[r], 0);
+    int len = max(p.len[r] + p.len_add, 0);
     // a padding row, or one that is refused: all threads of the item agree
     bool skip = seq < 0 || (WARP && index >= n_items);
     if (!skip && (seq >= g.n_seq || len > p.max_len ||
@@ -428,7 +445,6 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
         skip = true;
     }
     if (skip) len = 0;
-    int32_t* ctx = p.ctx + r * p.ldc + head0 * HD;
     const int me = WARP ? lane : tid, team = WARP ? 32 : blockDim.x;
     const int32_t* table = g.table + seq * g.ld_table;
     const int tiles = (len + 31) >> 5;
@@ -514,7 +530,7 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
     __syncthreads();
     if (len == 0) {
         if (!skip && rank == 0)
-            for (int i = me; i < nh * HD; i += team) ctx[i] = 0;
+            for (int i = me; i < nh * HD; i += team) store_context(p, r, head0 * HD + i, 0);
         return;
     }
     int use_s = 0;  // the ring's next tile to use
@@ -875,7 +891,7 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
                 }
                 if constexpr (BITS == 4) v += A == 1 || d < 64 ? pz[h][0] : pz[h][A - 1];
                 if (!WARP && cs > 1) ctx_s[h * HD + 64 * sweep + d] = v;
-                else ctx[h * HD + 64 * sweep + d] = static_cast<int32_t>(sat64(rs64(v, p.shift_c), p.bits_c));
+                else store_context(p, r, (head0 + h) * HD + 64 * sweep + d, v);
             }
         }
         if (!WARP && sweep + 1 < C::SWEEPS) __syncthreads();
@@ -887,7 +903,7 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
             for (int i = rank * blockDim.x + tid; i < nh * HD; i += cs * blockDim.x) {
                 int64_t v = 0;
                 for (int c = 0; c < cs; ++c) v += ld_remote64(remote_smem(ctx_s + i, c));
-                ctx[i] = static_cast<int32_t>(sat64(rs64(v, p.shift_c), p.bits_c));
+                store_context(p, r, head0 * HD + i, v);
             }
             cluster_barrier();  // no block leaves while its words are read
         }

@@ -276,7 +276,8 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
  *   s_j = SAT16(RS(q . k_j, shift_s)), e_j = E[max s - s_j] (0 beyond 1536), Z = sum e_j,
  *   P_j = floor((e_j 2^prob_bits + floor(Z / 2)) / Z),  ctx = SAT(RS(sum_j P_j v_j, shift_c), bits_c)
  * to ctx int32 rows of ldc elements.  prob_bits 16 gives the engine's attention; up to 19 keeps small
- * probabilities of long sequences.  shift_c = prob_bits + f_v - f_ctx.  len[r] <= 0 gives zeros;
+ * probabilities of long sequences.  shift_c = prob_bits + f_v - f_ctx in [-16, 62] (RS by n <= 0 is an
+ * exact left shift).  len[r] <= 0 gives zeros;
  * len[r] <= max_len <= EII_PAGED_MAX_LEN. */
 int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, int64_t ldq, int n_rows,
                         const int32_t* seq, const int32_t* len, int max_len, int shift_s, int prob_bits, int shift_c,
@@ -285,6 +286,28 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
 int eii_paged_sync(eii_paged* p, void* stream);
 /* The caller closes the handle after its last call has finished. */
 void eii_paged_close(eii_paged* p);
+
+/* Ragged decoding of the model on a paged cache (no reference counterpart): every row of a step is one
+ * token of sequence seq[r] at position pos[r] < 512, so prompts, parts of prompts and single tokens of
+ * many sequences go through the model together.  The decoder owns the pools of all layers (n_pages
+ * pages of page_size positions, cache_bits 16 or 4; 60 eii_paged_pool_bytes(n_pages) bytes); the
+ * caller hands out pages through the page table ([n_seq][ld_table] as in eii_pages, shared by all
+ * layers).  A step appends its rows, which then see positions 0 .. pos[r] of their sequence: rows of one
+ * sequence may come in one step, in ascending positions, and what lies before them has been appended
+ * by earlier steps.  At 16 bits the logits of a row equal the row of eii_forward on that prefix; at 4
+ * bits they are those of the compressed rows.  seq[r] < 0 (or pos[r] < 0) is padding: its id must be
+ * valid, its logits are undefined.  pos[r] < max_len <= 512 for every row.
+ * ids_dev int64, seq_dev, pos_dev, table_dev int32, logits_dev (nullable) int32 [n_rows][ld_logits] as in
+ * eii_forward_device.  Like eii_decoder_step_device_async the step returns once it is enqueued
+ * (null stream = the engine's), uses the engine's workspace, and leaves device-side errors to
+ * eii_paged_decoder_sync, after which the rows of the failed steps have to be appended again. */
+typedef struct eii_paged_decoder eii_paged_decoder;
+int eii_paged_decoder_open(eii_engine* e, int page_size, int cache_bits, int64_t n_pages, eii_paged_decoder** out);
+int eii_paged_decoder_step_device_async(eii_paged_decoder* d, const int64_t* ids_dev, const int32_t* seq_dev,
+                                        const int32_t* pos_dev, int n_rows, const int32_t* table_dev, int64_t ld_table,
+                                        int n_seq, int max_len, int32_t* logits_dev, int64_t ld_logits, void* stream);
+int eii_paged_decoder_sync(eii_paged_decoder* d, void* stream);
+void eii_paged_decoder_close(eii_paged_decoder* d); /* before its engine */
 
 /* Drawing the next tokens from integer logits and given random words, all in integers (no reference
  * counterpart).  Row r of logits (int32, exponent 16 as eii_forward writes them, ld elements apart,

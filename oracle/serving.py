@@ -148,3 +148,32 @@ def draw(row, u, inv_temp=65536, top_k=0, top_p=65536, min_p=0):
         if run > target:
             return int(i), order.size, (int(w[i]) * (1 << 30) + mass // 2) // mass
     raise AssertionError("the target lies below the mass")
+
+
+# ----------------------------------------------------------------------------- the model, 4-bit cache
+def forward_compressed(mdl, ids):
+    """Logits [T, V] of the forward pass (oracle.forward.forward) of one sequence whose k and v rows are kept
+    at 4 bits: the rows of every position, its own included, are what their nibbles stand for."""
+    from oracle import forward as ofw
+    ids = np.asarray(ids, I64)
+    T = ids.shape[0]
+
+    def stored(x):
+        out = np.empty_like(x)
+        for t in range(T):
+            for h in range(x.shape[1]):
+                n, m, z = quantise(x[t, h])
+                out[t, h] = z + m * n
+        return out
+    x = ofw.embed(mdl, ids)
+    plain = ofw.attention
+
+    def attention(qr, kr, v, *args, **kw):
+        return plain(qr, stored(kr), stored(v), *args, **kw)
+    try:
+        ofw.attention = attention
+        for l in range(len(mdl["layers"])):
+            x = ofw.block_batch(mdl, l, x, T)
+    finally:
+        ofw.attention = plain
+    return ofw.logits_from_y(mdl, ofw.final_norm(mdl, x))

@@ -221,6 +221,8 @@ def test_attention_extremes(torch, bits):
             check_attention(torch, c, rng, [0], [n], 150, shift_s=shift_s, q=q)
             check_attention(torch, c, rng, [0], [n], 150, shift_s=shift_s, q=q, pb=19, shift_c=1, bits_c=32)
             check_attention(torch, c, rng, [0], [n], 150, shift_s=shift_s, q=q, pb=19, shift_c=30, bits_c=2)
+            check_attention(torch, c, rng, [0], [n], 150, shift_s=shift_s, q=q, shift_c=-16, bits_c=32)
+            check_attention(torch, c, rng, [0], [n], 150, shift_s=shift_s, q=q, shift_c=0, bits_c=32)
 
 
 def test_attention_shared_pages(torch):
@@ -285,7 +287,7 @@ def test_cache_refusals(torch):
                 lambda: append(shift_k=63), lambda: append(ldk=191), lambda: append(q_ptr=q.data_ptr()),
                 lambda: append(q_out_ptr=q.data_ptr()), lambda: append(q_ptr=q.data_ptr(), q_out_ptr=q.data_ptr(), shift_q=0),
                 lambda: attend(n=3), lambda: attend(max_len=131073), lambda: attend(max_len=-1), lambda: attend(prob_bits=15),
-                lambda: attend(prob_bits=20), lambda: attend(shift_s=0), lambda: attend(shift_c=63), lambda: attend(bits_c=33),
+                lambda: attend(prob_bits=20), lambda: attend(shift_s=0), lambda: attend(shift_c=63), lambda: attend(shift_c=-17), lambda: attend(bits_c=33),
                 lambda: attend(ldq=575), lambda: attend(ldc=575), lambda: c.p.pool_bytes(0)):
         with pytest.raises(_eii.EiiError) as e:
             bad()
