@@ -84,21 +84,22 @@ __device__ __forceinline__ uint64_t sample_target(uint64_t mass, uint32_t u) {
 //
 // The kept tokens are a prefix of the order (weight descending, index ascending): all weights above theta
 // and the first `quota` of those equal to it.  A cut is found by narrowing a window [lo, hi) around it:
-// with passes over the row, the first two at places that a sample of the row suggests, until the window is
+// with passes over the row, the first at places that a sample of the row suggests, until the window is
 // short enough for a list; with passes over that list; and, from SAMPLE_FEW on, by comparing each with all.
-// Every decision rests on exact sums; the sample only chooses where to look.  A list that holds all kept
-// weights serves the draw too.
+// Every decision rests on exact sums; the sample only chooses where to look.  Each thread knows the mass of
+// its own weights above the window, and its entries of the list are contiguous, so the draw needs no
+// further pass: a row is read for its maximum, for the weights, and once or twice for the cut.
 constexpr int SAMPLE_THREADS = 1024, SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_MAX_CLUSTER = 16, SAMPLE_MAX_CHUNKS = 12;
 constexpr int SAMPLE_GUESS_CHUNKS = 6;
-constexpr int SAMPLE_LIST = 4096, SAMPLE_FEW = 64;
+constexpr int SAMPLE_LIST = 8192, SAMPLE_FEW = 64;
 constexpr uint32_t SAMPLE_TOP = (1u << 30) + 1;  // above every weight
 
 // Words that the threads of a block (and the blocks of a cluster) exchange come in two sets that take turns,
 // so that one is not overwritten before its slowest reader has it: a barrier lies between the uses of a set.
 struct SampleShared {
-    uint32_t w[SAMPLE_LIST], i[SAMPLE_LIST];  // the list; of a cluster's blocks the first half, the second for all
-    alignas(8) uint32_t few[SAMPLE_FEW];
+    uint32_t w[SAMPLE_LIST];  // the list; of a cluster's blocks the first half, the second for all
+    uint32_t few[SAMPLE_FEW];
     int32_t warp_max[2][SAMPLE_WARPS];
     uint64_t warp_mass[2][SAMPLE_WARPS];
     uint32_t warp_n[2][SAMPLE_WARPS];
@@ -166,22 +167,24 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         }
         cp_async_commit();
     };
-    // sums over the block's threads, in every thread
-    auto total = [&](uint64_t& m, uint32_t& n) {
+    // sums over the threads of the block's first `warps` warps, in every thread
+    auto total = [&](uint64_t& m, uint32_t& n, int warps) {
         turn ^= 1;
-        m = warp_sum47(m);
-        n = __reduce_add_sync(~0u, n);
-        if (lane == 0) {
-            sh.warp_mass[turn][warp] = m;
-            sh.warp_n[turn][warp] = n;
+        if (warp < warps) {
+            m = warp_sum47(m);
+            n = __reduce_add_sync(~0u, n);
+            if (lane == 0) {
+                sh.warp_mass[turn][warp] = m;
+                sh.warp_n[turn][warp] = n;
+            }
         }
         __syncthreads();
-        m = warp_sum47(sh.warp_mass[turn][lane]);
-        n = __reduce_add_sync(~0u, sh.warp_n[turn][lane]);
+        m = warp_sum47(lane < warps ? sh.warp_mass[turn][lane] : 0);
+        n = __reduce_add_sync(~0u, lane < warps ? sh.warp_n[turn][lane] : 0);
     };
     // ... and over the cluster's
     auto total_cluster = [&](uint64_t& m, uint32_t& n) {
-        total(m, n);
+        total(m, n, SAMPLE_WARPS);
         if (cs > 1) {
             if (tid == 0) {
                 sh.block_mass[turn] = m;
@@ -261,8 +264,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
             continue;
         }
         // Weights.  min-p first, whose cut is known: weights below it go.  (All three keep prefixes of one order.)
-        uint64_t mass = 0;
-        uint32_t n = 0, some = 0;
+        uint64_t own_mass = 0;
+        uint32_t own_n = 0, some = 0;
         const uint32_t least = max(static_cast<uint32_t>(q.mp) << 14, 1u);
         auto weigh_all = [&](auto with_min) {
             each([&](int k, uint4* x) {
@@ -270,30 +273,34 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 auto weigh = [&](uint32_t l) {
                     const uint32_t w = sample_weight(static_cast<int32_t>(l), mx, q.b2);
                     if (!decltype(with_min)::value) {
-                        n += w != 0;
+                        own_n += w != 0;
                         return w;
                     }
-                    n += w >= least;
+                    own_n += w >= least;
                     return w >= least ? w : 0;
                 };
                 v = make_uint4(weigh(v.x), weigh(v.y), weigh(v.z), weigh(v.w));
                 *x = v;
-                mass += v.x + v.y;  // (at most 2^31)
-                mass += v.z + v.w;
+                own_mass += v.x + v.y;  // (at most 2^31)
+                own_mass += v.z + v.w;
                 if (k == ch >> 1) some = v.x;
             });
         };
         if (q.mp) weigh_all(std::true_type{});
         else weigh_all(std::false_type{});
+        uint64_t mass = own_mass;
+        uint32_t n = own_n;
         total_cluster(mass, n);
 
         // theta, the mass and the number of the weights above it, and how many equal to it are kept
         uint32_t theta = 0, above_n = n;
         uint64_t above = mass, quota = 0;
-        uint32_t list_n = 0;
-        bool listed = false;  // the list holds all that is kept
-        const uint32_t* lw = sh.w;
-        const uint32_t* li = sh.i;
+        // the list: its length, what this thread has of it and above it, and whether anything is above it
+        uint32_t list_n = 0, mine_at = 0, mine_n = 0;
+        uint64_t mine_above = own_mass;
+        bool have_list = false, list_to_top = false, by_row = false;
+        const uint32_t* lw = cs > 1 ? sh.w + SAMPLE_LIST / 2 : sh.w;
+        const uint32_t room = cs > 1 ? SAMPLE_LIST / 2 : SAMPLE_LIST;
 #pragma unroll 1
         for (int stage = 0; stage < 2; ++stage) {
             const bool by_count = stage == 0;  // top-k, then top-p
@@ -311,7 +318,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 }
             }
             // The largest theta whose weights >= theta number or weigh `goal` lies in [lo, hi), where c weights (at most)
-            // are; hi_mass and hi_n are above.  Weights up to (above - goal) / vocab, all together, are not missed.
+            // are; hi_mass and hi_n are at or above hi.  Weights up to (above - goal) / vocab, all together, are not missed.
             uint32_t lo = theta + 1, hi = SAMPLE_TOP, hi_n = 0, c = above_n;
             uint64_t hi_mass = 0;
             if (!by_count) lo = max(lo, static_cast<uint32_t>((above - goal) / static_cast<uint32_t>(p.vocab)) + 1);
@@ -319,80 +326,68 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 if (hi > 4 * lo) return 1u << ((63 - __clz(lo) - __clz(hi)) / 2);  // (between: their lengths differ by two)
                 return lo + (hi - lo) / 2;
             };
-            // narrows the window to [mid, hi), with mass m and x weights, or to [lo, mid)
+            // narrows the window to [mid, hi), with mass m and x weights, or to [lo, mid); true for the first
             auto narrow = [&](uint32_t mid, uint64_t m, uint32_t x) {
                 if ((by_count ? hi_n + x : hi_mass + m) >= goal) {
                     lo = mid;
                     c = x;
-                } else {
-                    hi = mid;
-                    hi_mass += m;
-                    hi_n += x;
-                    c -= x;
+                    return true;
                 }
+                hi = mid;
+                hi_mass += m;
+                hi_n += x;
+                c -= x;
+                return false;
             };
-            if (!listed) {
-                const uint32_t room = cs > 1 ? SAMPLE_LIST / 2 : SAMPLE_LIST;
+            if (!(have_list && list_to_top)) {
                 // Where to look first.  For a count: the greatest of 1024 thresholds that `goal` threads' largest weights
                 // reach, which as many weights then do.  For a mass: a sample of one weight per thread tells where the
-                // mass that may be missed, less and more a quarter, is expected to lie below.  (Not worth it where a pass
-                // is short: one row of 49152 on four blocks takes 20 us without and 25 with.)
-                uint32_t guess_lo = 0, guess_hi = 0;
+                // mass that may be missed is expected to lie below.  (Not worth it where a pass is short: one row of 49152
+                // on four blocks takes 20 us without and 25 with.)
+                uint32_t guess = 0;
                 if (c > room && ch >= SAMPLE_GUESS_CHUNKS && (!by_count || goal <= SAMPLE_THREADS / 2)) {
                     const uint32_t top = sample_weight(own_max, mx, q.b2);
                     sh.w[tid] = by_count ? (top >= least ? top : 0) : some;
                     __syncthreads();
-                    uint32_t at[2] = {0, 0}, unit[2] = {1, 1};
-                    const uint64_t scale = 4 * ch * cs, want = by_count ? goal : above - goal;
+                    const uint64_t want = by_count ? goal : (above - goal) / static_cast<uint32_t>(4 * ch * cs);
+                    uint32_t unit = 1;
 #pragma unroll 1
                     for (int round = 0; round < 2; ++round) {
-                        // warp b's threshold: the octave 2^b, then its 32nd parts
-                        const uint32_t th0 = round == 0 ? 1u << warp : at[0] + warp * unit[0];
-                        const uint32_t th1 = round == 0 ? 1u << warp : at[1] + warp * unit[1];
-                        uint64_t f0 = 0, f1 = 0;
-#pragma unroll 4
+                        // warp b's threshold: the octave 2^b, then its 32nd parts; masses in units of 2^11
+                        const uint32_t th = round == 0 ? 1u << warp : guess + warp * unit;
+                        uint32_t f = 0;
+#pragma unroll 8
                         for (int i = lane; i < SAMPLE_THREADS; i += 32) {
                             const uint32_t w = sh.w[i];
-                            if (by_count) f0 += w >= th0;
-                            else {
-                                f0 += w < th0 ? w : 0;
-                                f1 += w < th1 ? w : 0;
-                            }
+                            if (by_count) f += w >= th;
+                            else f += w < th ? (w + 1024) >> 11 : 0;
                         }
-                        f0 = warp_sum47(f0);
-                        f1 = warp_sum47(f1);
+                        f = __reduce_add_sync(~0u, f);
                         turn ^= 1;
-                        if (lane == 0) {
-                            sh.warp_mass[turn][warp] = f0;
-                            reinterpret_cast<uint64_t*>(sh.few)[warp] = f1;
-                        }
+                        if (lane == 0) sh.warp_n[turn][warp] = f;
                         __syncthreads();
-                        f0 = sh.warp_mass[turn][lane];
-                        f1 = reinterpret_cast<const uint64_t*>(sh.few)[lane];
-                        const bool in0 = by_count ? f0 >= want : 4 * scale * f0 <= 3 * want;  // (true up to some threshold)
-                        const bool in1 = 4 * scale * f1 <= 5 * want;
-                        const int b0 = 31 - __clz(__ballot_sync(~0u, in0)), b1 = 31 - __clz(__ballot_sync(~0u, in1));
-                        at[0] = round == 0 ? 1u << max(b0, 0) : at[0] + max(b0, 0) * unit[0];
-                        at[1] = round == 0 ? 1u << max(b1, 0) : at[1] + max(b1, 0) * unit[1];
-                        unit[0] = max(at[0] >> 5, 1u);
-                        unit[1] = max(at[1] >> 5, 1u);
-                        if (by_count && b0 < 0) at[0] = 0;  // (fewer threads than that have any weight)
-                        __syncthreads();
+                        f = sh.warp_n[turn][lane];
+                        // (true up to some threshold)
+                        const int b = 31 - __clz(__ballot_sync(~0u, by_count ? f >= want : static_cast<uint64_t>(f) << 11 <= want));
+                        guess = round == 0 ? 1u << max(b, 0) : guess + max(b, 0) * unit;
+                        unit = max(guess >> 5, 1u);
+                        if (by_count && b < 0) guess = 0;  // (fewer threads than that have any weight)
                     }
-                    guess_lo = at[0];
-                    guess_hi = by_count ? 0 : at[1] + unit[1];
                     if (cs > 1) {  // the first block's guess is the cluster's
                         turn ^= 1;
-                        if (tid == 0) {
-                            sh.block_n[turn] = guess_lo;
-                            sh.block_mass[turn] = guess_hi;
-                        }
+                        if (tid == 0) sh.block_n[turn] = guess;
                         cluster_barrier();
-                        guess_lo = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], 0)));
-                        guess_hi = static_cast<uint32_t>(ld_remote64(remote_smem(&sh.block_mass[turn], 0)));
+                        guess = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], 0)));
                     }
                 }
-                auto pass = [&](uint32_t mid) {
+                // this thread's weights in [lo, hi) (once known) and at or above hi
+                uint32_t in_n = 0, up_n = 0;
+                uint64_t up_mass = 0;
+                bool known = false;
+                for (int k = 0; c > room && hi - lo > 1; ++k) {
+                    // around a guessed mass first a fifth below, then a quarter above
+                    uint32_t mid = k == 0 ? (by_count ? guess : guess - guess / 5) : k == 1 && !by_count ? guess + guess / 4 : 0;
+                    if (mid <= lo || mid >= hi) mid = middle();
                     uint64_t m = 0;
                     uint32_t x = 0;
                     each([&](int, uint4* at) {
@@ -404,53 +399,52 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                         m += y;
                         m += z;
                     });
+                    const uint64_t own_m = m;
+                    const uint32_t own_x = x;
                     total_cluster(m, x);
-                    narrow(mid, m - hi_mass, x - hi_n);
-                };
-                for (int k = 0; c > room && hi - lo > 1; ++k) {
-                    const uint32_t guess = k == 0 ? guess_lo : k == 1 ? guess_hi : 0;
-                    pass(guess > lo && guess < hi ? guess : middle());
+                    if (narrow(mid, m - hi_mass, x - hi_n)) {
+                        in_n = own_x - up_n;
+                        known = true;
+                    } else {
+                        in_n -= own_x - up_n;
+                        up_n = own_x;
+                        up_mass = own_m;
+                    }
                 }
-                if (hi - lo > 1) {
-                    // the window's weights and indices, in index order
-                    uint32_t x = 0;
-                    each([&](int, uint4* at) {
-                        const uint4 v = *at;
-                        x += (v.x - lo < hi - lo) + (v.y - lo < hi - lo) + (v.z - lo < hi - lo) + (v.w - lo < hi - lo);
-                    });
+                by_row = hi - lo == 1;  // (the cut fell on the way: the draw counts the row again)
+                if (!by_row) {
+                    // the window's weights, by thread
+                    if (!known) {
+                        in_n = 0;
+                        each([&](int, uint4* at) {
+                            const uint4 v = *at;
+                            in_n += (v.x - lo < hi - lo) + (v.y - lo < hi - lo) + (v.z - lo < hi - lo) + (v.w - lo < hi - lo);
+                        });
+                    }
                     uint64_t none;
-                    uint32_t at;
-                    before(0, x, false, none, at);
-                    if (x)
-                        each([&](int k, uint4* from) {
+                    before(0, in_n, false, none, mine_at);
+                    mine_n = in_n;
+                    mine_above = up_mass;
+                    uint32_t at = mine_at;
+                    if (in_n)
+                        each([&](int, uint4* from) {
                             const uint4 v = *from;
-                            auto put = [&](uint32_t w, int j) {
-                                if (w - lo < hi - lo) {
-                                    sh.w[at] = w;
-                                    sh.i[at] = base + 4 * k + j;
-                                    ++at;
-                                }
-                            };
-                            put(v.x, 0);
-                            put(v.y, 1);
-                            put(v.z, 2);
-                            put(v.w, 3);
+                            if (v.x - lo < hi - lo) sh.w[at++] = v.x;
+                            if (v.y - lo < hi - lo) sh.w[at++] = v.y;
+                            if (v.z - lo < hi - lo) sh.w[at++] = v.z;
+                            if (v.w - lo < hi - lo) sh.w[at++] = v.w;
                         });
                     if (cs > 1) {
                         if (tid == SAMPLE_THREADS - 1) sh.block_n[turn] = at;
                         cluster_barrier();
-                        uint32_t to = 0;
+                        uint32_t to = SAMPLE_LIST / 2;
                         for (int b = 0; b < cs; ++b) {
                             const uint32_t have = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], b)));
-                            for (uint32_t i = tid; i < have; i += SAMPLE_THREADS) {
-                                sh.w[SAMPLE_LIST / 2 + to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.w[i], b)));
-                                sh.i[SAMPLE_LIST / 2 + to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.i[i], b)));
-                            }
+                            for (uint32_t i = tid; i < have; i += SAMPLE_THREADS)
+                                sh.w[to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.w[i], b)));
                             to += have;
                         }
-                        list_n = to;
-                        lw = sh.w + SAMPLE_LIST / 2;
-                        li = sh.i + SAMPLE_LIST / 2;
+                        list_n = to - SAMPLE_LIST / 2;
                         cluster_barrier();
                     } else {
                         if (tid == SAMPLE_THREADS - 1) sh.few_n = at;
@@ -458,31 +452,35 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                         list_n = sh.few_n;
                     }
                     c = list_n;
-                    listed = hi == SAMPLE_TOP;
+                    have_list = true;
+                    list_to_top = hi == SAMPLE_TOP;
                 }
             }
+            const int busy = min(static_cast<int>(list_n + 127) / 128, SAMPLE_WARPS);  // warps that share the list
             while (c > SAMPLE_FEW && hi - lo > 1) {
                 const uint32_t mid = middle();
                 uint64_t m = 0;
                 uint32_t x = 0;
-                for (uint32_t i = tid; i < list_n; i += SAMPLE_THREADS) {
-                    const uint32_t w = lw[i];
-                    if (w - mid < hi - mid) {
-                        m += w;
-                        ++x;
+                if (warp < busy)
+                    for (uint32_t i = tid; i < list_n; i += 32 * busy) {
+                        const uint32_t w = lw[i];
+                        if (w - mid < hi - mid) {
+                            m += w;
+                            ++x;
+                        }
                     }
-                }
-                total(m, x);
+                total(m, x, busy);
                 narrow(mid, m, x);
             }
             if (hi - lo > 1) {
                 __syncthreads();
                 if (tid == 0) sh.few_n = 0;
                 __syncthreads();
-                for (uint32_t i = tid; i < list_n; i += SAMPLE_THREADS) {
-                    const uint32_t w = lw[i];
-                    if (w - lo < hi - lo) sh.few[atomicAdd(&sh.few_n, 1u)] = w;
-                }
+                if (warp < busy)
+                    for (uint32_t i = tid; i < list_n; i += 32 * busy) {
+                        const uint32_t w = lw[i];
+                        if (w - lo < hi - lo) sh.few[atomicAdd(&sh.few_n, 1u)] = w;
+                    }
                 __syncthreads();
                 const uint32_t few_n = sh.few_n;
                 // warp b: candidates b, b + 32, ...
@@ -523,36 +521,30 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         }
         const uint64_t target = sample_target(mass, u);
 
-        // The draw: kept mass and ties of each thread's part of the list or of the row, in index order.
-        uint64_t m = 0;
+        // The draw: kept mass and ties of each thread's part of the row, in index order.
+        uint64_t m = mine_above;
         uint32_t t = 0;
-        uint32_t i0 = 0, i1 = 0;
-        if (listed) {
-            const uint32_t per = (list_n + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
-            i0 = min(tid * per, list_n);
-            i1 = min(i0 + per, list_n);
-            for (uint32_t i = i0; i < i1; ++i) {
-                const uint32_t w = lw[i];
+        if (by_row) {
+            m = 0;
+            each([&](int, uint4* at) {
+                const uint4 v = *at;
+                m += (v.x > theta ? v.x : 0) + (v.y > theta ? v.y : 0);
+                m += (v.z > theta ? v.z : 0) + (v.w > theta ? v.w : 0);
+                t += (v.x == theta) + (v.y == theta) + (v.z == theta) + (v.w == theta);
+            });
+        } else if (have_list) {
+            for (uint32_t i = mine_at; i < mine_at + mine_n; ++i) {
+                const uint32_t w = sh.w[i];
                 m += w > theta ? w : 0;
                 t += w == theta;
             }
-        } else {
-            each([&](int, uint4* at) {
-                const uint4 v = *at;
-                uint32_t y = v.x > theta ? v.x : 0, z = v.z > theta ? v.z : 0;
-                t += (v.x == theta) + (v.y == theta) + (v.z == theta) + (v.w == theta);
-                y += v.y > theta ? v.y : 0;
-                z += v.w > theta ? v.w : 0;
-                m += y;
-                m += z;
-            });
         }
         uint64_t cur;
         uint32_t ties;
-        before(m, t, cs > 1 && !listed, cur, ties);
+        before(m, t, cs > 1, cur, ties);
         uint64_t used = ties;
         cur += theta * min(used, quota);
-        if (cur <= target && target < cur + m + theta * min(static_cast<uint64_t>(t), quota - min(quota, used)) && (!listed || rank == 0)) {
+        if (cur <= target && target < cur + m + theta * min(static_cast<uint64_t>(t), quota - min(quota, used))) {
             // one thread; its kept weights up to the target
             uint32_t won = 0;
             int at = -1;
@@ -565,16 +557,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                     cur += w;
                 }
             };
-            if (listed)
-                for (uint32_t i = i0; i < i1; ++i) look(lw[i], static_cast<int>(li[i]));
-            else
-                each([&](int k, uint4* from) {
-                    const uint4 v = *from;
-                    look(v.x, base + 4 * k);
-                    look(v.y, base + 4 * k + 1);
-                    look(v.z, base + 4 * k + 2);
-                    look(v.w, base + 4 * k + 3);
-                });
+            each([&](int k, uint4* from) {
+                const uint4 v = *from;
+                look(v.x, base + 4 * k);
+                look(v.y, base + 4 * k + 1);
+                look(v.z, base + 4 * k + 2);
+                look(v.w, base + 4 * k + 3);
+            });
             p.token[r] = at;
             if (p.kept) p.kept[r] = static_cast<int32_t>(above_n + quota);
             if (p.prob) p.prob[r] = static_cast<int32_t>(((static_cast<uint64_t>(won) << 30) + (mass >> 1)) / mass);
