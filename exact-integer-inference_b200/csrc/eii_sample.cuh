@@ -55,18 +55,26 @@ __device__ __forceinline__ SampleRow sample_row(const SampleParams& p, int r) {
     return o;
 }
 
-// floor(y f / 2^31) of the 31-bit fraction f is umulhi(y, 2 f); RS(y, n) = ((2 y >> n) + 1) >> 1.
-__device__ __forceinline__ uint32_t sample_weight(int32_t l, int32_t row_max, uint32_t b2) {
-    const uint64_t x = static_cast<uint64_t>(static_cast<uint32_t>(row_max) - static_cast<uint32_t>(l)) * b2;
-    const uint32_t hi = static_cast<uint32_t>(x >> 32);
-    const uint32_t f2 = __funnelshift_r(static_cast<uint32_t>(x), hi, 8) & 0xFFFFFF00u;
-    uint32_t y = SAMPLE_C3 - __umulhi(SAMPLE_C4, f2);
-    y = SAMPLE_C2 - __umulhi(y, f2);
-    y = SAMPLE_C1 - __umulhi(y, f2);
-    y = (1u << 31) - 2 * __umulhi(y, f2);
-    const uint32_t w = (__funnelshift_rc(y, 0, hi >> 8) + 1) >> 1;
-    return hi < (31u << 8) && l != SAMPLE_MASKED ? w : 0;
-}
+// A row's weights.
+struct SampleScale {
+    uint32_t row_max, b2;
+    // The polynomial runs on the double-precision pipe, the integer one being what bounds the kernel: u = f 2^-24
+    // exactly, and y u + 2^52 rounded down is 2^52 + floor(y u) for every y below 2^30 (one rounding, at the units'
+    // place).  RS(y, n) = ((2 y >> n) + 1) >> 1.
+    __device__ __forceinline__ uint32_t operator()(uint32_t logit) const {
+        const uint64_t x = static_cast<uint64_t>(row_max - logit) * b2;
+        const uint32_t hi = static_cast<uint32_t>(x >> 32), lo = static_cast<uint32_t>(x);
+        constexpr double M = 4503599627370496.0;  // 2^52
+        const double u = __hiloint2double(static_cast<int>((__funnelshift_r(lo, hi, 20) & 0xFFFFFu) | 0x3FF00000u),
+                                          static_cast<int>((lo << 12) & 0xF0000000u)) - 1.0;
+        double y = (M + SAMPLE_C3) - __fma_rd(static_cast<double>(SAMPLE_C4), u, M);
+        y = (M + SAMPLE_C2) - __fma_rd(y, u, M);
+        y = (M + SAMPLE_C1) - __fma_rd(y, u, M);
+        const uint32_t k = static_cast<uint32_t>(__double2loint(__fma_rd(y, u, M)));
+        const uint32_t w = (__funnelshift_rc((1u << 31) - 2 * k, 0, hi >> 8) + 1) >> 1;
+        return hi < (31u << 8) && logit != static_cast<uint32_t>(SAMPLE_MASKED) ? w : 0;
+    }
+};
 
 // ceil(p mass / 2^16), at least 1.
 __device__ __forceinline__ uint64_t sample_goal(uint64_t mass, int p) {
@@ -118,50 +126,41 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
     const int rank = cs > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int base = (rank * SAMPLE_THREADS + tid) * 4 * ch;  // this thread's first logit
     const int step = gridDim.x / cs;
-    // A thread's chunk k lies at (k + shift) mod ch of its ch places: where ch is even, eight neighbours start on
-    // eight banks.
-    auto shift_of = [&](int l) {
-        int x = ch & 1 ? 0 : l & 7;
-        while (x >= ch) x -= ch;
-        return x;
-    };
-    const int shift = shift_of(lane);
     uint4* warp_buf = reinterpret_cast<uint4*>(smem) + warp * 32 * ch;
     uint4* buf = warp_buf + lane * ch;
+    // A thread goes through its chunks from one that depends on its lane on, so that where ch is even eight
+    // neighbours read from eight banks.
+    int start = ch & 1 ? 0 : lane & 7;
+    while (start >= ch) start -= ch;
     int turn = 0;
 
-    // f(chunk's number, its place) over this thread's chunks, in index order
+    // f(number of a chunk, the chunk) over this thread's chunks
     auto each = [&](auto f) {
-        int place = shift;
+        int k = start;
 #pragma unroll 4
-        for (int k = 0; k < ch; ++k) {
-            f(k, buf + place);
-            place = place + 1 == ch ? 0 : place + 1;
+        for (int i = 0; i < ch; ++i) {
+            f(k, buf + k);
+            k = k + 1 == ch ? 0 : k + 1;
         }
     };
     // this warp's part of row r to shared memory, masked behind the row's end
+    const int first = base - lane * 4 * ch;  // the warp's first logit
+    const bool whole = aligned && p.vocab - first >= 128 * ch;
     auto copy = [&](int r) {
         if (r < p.n_rows) {
-            const int at = base - lane * 4 * ch;  // the warp's first logit
-            const int32_t* row = p.logits + r * p.ld + at;
-            int owner = lane / ch, k = lane - owner * ch;
-            const int step_o = 32 / ch, step_k = 32 - step_o * ch;
+            const int32_t* row = p.logits + r * p.ld + first;
+            if (whole) {
 #pragma unroll 4
-            for (int c = lane; c < 32 * ch; c += 32) {
-                const int place = k + shift_of(owner);
-                uint4* dst = warp_buf + owner * ch + (place >= ch ? place - ch : place);
-                const int left = p.vocab - at - 4 * c;
-                if (aligned && left >= 4) cp_async16(dst, row + 4 * c);
-                else
-                    for (int j = 0; j < 4; ++j) {
-                        if (j < left) cp_async4(reinterpret_cast<uint32_t*>(dst) + j, row + 4 * c + j);
-                        else reinterpret_cast<int32_t*>(dst)[j] = SAMPLE_MASKED;
-                    }
-                owner += step_o;
-                k += step_k;
-                if (k >= ch) {
-                    k -= ch;
-                    ++owner;
+                for (int c = lane; c < 32 * ch; c += 32) cp_async16(warp_buf + c, row + 4 * c);
+            } else {
+                for (int c = lane; c < 32 * ch; c += 32) {
+                    const int left = p.vocab - first - 4 * c;
+                    if (aligned && left >= 4) cp_async16(warp_buf + c, row + 4 * c);
+                    else
+                        for (int j = 0; j < 4; ++j) {
+                            if (j < left) cp_async4(reinterpret_cast<uint32_t*>(warp_buf + c) + j, row + 4 * c + j);
+                            else reinterpret_cast<int32_t*>(warp_buf + c)[j] = SAMPLE_MASKED;
+                        }
                 }
             }
         }
@@ -264,6 +263,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
             continue;
         }
         // Weights.  min-p first, whose cut is known: weights below it go.  (All three keep prefixes of one order.)
+        const SampleScale scale{static_cast<uint32_t>(mx), q.b2};
         uint64_t own_mass = 0;
         uint32_t own_n = 0, some = 0;
         const uint32_t least = max(static_cast<uint32_t>(q.mp) << 14, 1u);
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
             each([&](int k, uint4* x) {
                 uint4 v = *x;
                 auto weigh = [&](uint32_t l) {
-                    const uint32_t w = sample_weight(static_cast<int32_t>(l), mx, q.b2);
+                    const uint32_t w = scale(l);
                     if (!decltype(with_min)::value) {
                         own_n += w != 0;
                         return w;
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 };
                 v = make_uint4(weigh(v.x), weigh(v.y), weigh(v.z), weigh(v.w));
                 *x = v;
-                own_mass += v.x + v.y;  // (at most 2^31)
+                own_mass += v.x + v.y;  // (two are at most 2^31)
                 own_mass += v.z + v.w;
                 if (k == ch >> 1) some = v.x;
             });
@@ -291,6 +291,17 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         uint64_t mass = own_mass;
         uint32_t n = own_n;
         total_cluster(mass, n);
+        // Once a warp needs its part of the row no more, the next row's may come.
+        bool released = false;
+        auto release = [&]() {
+            if (!released) {
+                __syncwarp();
+                copy(r + step);
+                released = true;
+            }
+        };
+        const bool cuts_n = q.k != 0 && static_cast<uint32_t>(q.k) < n, cuts_mass = q.p < 65536;
+        if (!cuts_n && !cuts_mass) release();
 
         // theta, the mass and the number of the weights above it, and how many equal to it are kept
         uint32_t theta = 0, above_n = n;
@@ -306,10 +317,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
             const bool by_count = stage == 0;  // top-k, then top-p
             uint64_t goal;
             if (by_count) {
-                if (q.k == 0 || static_cast<uint32_t>(q.k) >= n) continue;
+                if (!cuts_n) continue;
                 goal = q.k;
             } else {
-                if (q.p >= 65536) continue;
+                if (!cuts_mass) continue;
                 goal = sample_goal(mass, q.p);
                 if (above < goal) {  // (within the ties that top-k kept)
                     quota = (goal - above + theta - 1) / theta;
@@ -346,21 +357,21 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 // on four blocks takes 20 us without and 25 with.)
                 uint32_t guess = 0;
                 if (c > room && ch >= SAMPLE_GUESS_CHUNKS && (!by_count || goal <= SAMPLE_THREADS / 2)) {
-                    const uint32_t top = sample_weight(own_max, mx, q.b2);
-                    sh.w[tid] = by_count ? (top >= least ? top : 0) : some;
+                    const uint32_t top = scale(own_max);
+                    sh.w[tid] = by_count ? (top >= least ? top : 0) : (some + 1024) >> 11;  // (masses in units of 2^11)
                     __syncthreads();
                     const uint64_t want = by_count ? goal : (above - goal) / static_cast<uint32_t>(4 * ch * cs);
                     uint32_t unit = 1;
 #pragma unroll 1
                     for (int round = 0; round < 2; ++round) {
-                        // warp b's threshold: the octave 2^b, then its 32nd parts; masses in units of 2^11
-                        const uint32_t th = round == 0 ? 1u << warp : guess + warp * unit;
+                        // warp b's threshold: the octave 2^b, then its 32nd parts
+                        const uint32_t th = round == 0 ? 1u << warp : guess + warp * unit, th11 = (th + 1024) >> 11;
                         uint32_t f = 0;
-#pragma unroll 8
-                        for (int i = lane; i < SAMPLE_THREADS; i += 32) {
-                            const uint32_t w = sh.w[i];
-                            if (by_count) f += w >= th;
-                            else f += w < th ? (w + 1024) >> 11 : 0;
+#pragma unroll
+                        for (int i = lane; i < SAMPLE_THREADS / 4; i += 32) {
+                            const uint4 w = reinterpret_cast<const uint4*>(sh.w)[i];
+                            if (by_count) f += (w.x >= th) + (w.y >= th) + (w.z >= th) + (w.w >= th);
+                            else f += (w.x < th11 ? w.x : 0) + (w.y < th11 ? w.y : 0) + (w.z < th11 ? w.z : 0) + (w.w < th11 ? w.w : 0);
                         }
                         f = __reduce_add_sync(~0u, f);
                         turn ^= 1;
@@ -391,14 +402,20 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                     uint64_t m = 0;
                     uint32_t x = 0;
                     each([&](int, uint4* at) {
+                        // max(v, mid) summed, and how often it is above max(v, mid - 1), which tells the others
                         const uint4 v = *at;
-                        uint32_t y = v.x >= mid ? v.x : 0, z = v.z >= mid ? v.z : 0;
-                        x += (v.x >= mid) + (v.y >= mid) + (v.z >= mid) + (v.w >= mid);
-                        y += v.y >= mid ? v.y : 0;
-                        z += v.w >= mid ? v.w : 0;
-                        m += y;
-                        m += z;
+                        auto add = [&](uint32_t w) {
+                            const uint32_t a = max(w, mid), b = max(w, mid - 1);
+                            m += a;
+                            x += a - b;
+                        };
+                        add(v.x);
+                        add(v.y);
+                        add(v.z);
+                        add(v.w);
                     });
+                    m -= static_cast<uint64_t>(mid) * x;  // (x weights lie below mid)
+                    x = 4 * ch - x;
                     const uint64_t own_m = m;
                     const uint32_t own_x = x;
                     total_cluster(m, x);
@@ -454,6 +471,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                     c = list_n;
                     have_list = true;
                     list_to_top = hi == SAMPLE_TOP;
+                    if (list_to_top || !by_count || !cuts_mass) release();
                 }
             }
             const int busy = min(static_cast<int>(list_n + 127) / 128, SAMPLE_WARPS);  // warps that share the list
@@ -473,24 +491,32 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 narrow(mid, m, x);
             }
             if (hi - lo > 1) {
-                __syncthreads();
-                if (tid == 0) sh.few_n = 0;
-                __syncthreads();
-                if (warp < busy)
-                    for (uint32_t i = tid; i < list_n; i += 32 * busy) {
-                        const uint32_t w = lw[i];
-                        if (w - lo < hi - lo) sh.few[atomicAdd(&sh.few_n, 1u)] = w;
-                    }
-                __syncthreads();
-                const uint32_t few_n = sh.few_n;
-                // warp b: candidates b, b + 32, ...
+                const uint32_t* few = lw;
+                uint32_t few_n = list_n;
+                if (list_n > SAMPLE_FEW) {
+                    __syncthreads();
+                    if (tid == 0) sh.few_n = 0;
+                    __syncthreads();
+                    if (warp < busy)
+                        for (uint32_t i = tid; i < list_n; i += 32 * busy) {
+                            const uint32_t w = lw[i];
+                            if (w - lo < hi - lo) sh.few[atomicAdd(&sh.few_n, 1u)] = w;
+                        }
+                    __syncthreads();
+                    few = sh.few;
+                    few_n = sh.few_n;
+                } else if (!by_count) {
+                    __syncthreads();  // (top-k's words have been read)
+                }
+                // warp b: candidates b, b + 32, ... (a short list as it is may hold weights outside the window)
                 for (uint32_t j = warp; j < few_n; j += SAMPLE_WARPS) {
-                    const uint32_t mine = sh.few[j];
+                    const uint32_t mine = few[j];
+                    if (mine - lo >= hi - lo) continue;
                     uint64_t m = 0;  // of those above mine
                     uint32_t x = 0, same = 0;
                     for (uint32_t i = lane; i < few_n; i += 32) {
-                        const uint32_t w = sh.few[i];
-                        if (w > mine) {
+                        const uint32_t w = few[i];
+                        if (w > mine && w < hi) {
                             m += w;
                             ++x;
                         }
@@ -544,32 +570,36 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         before(m, t, cs > 1, cur, ties);
         uint64_t used = ties;
         cur += theta * min(used, quota);
-        if (cur <= target && target < cur + m + theta * min(static_cast<uint64_t>(t), quota - min(quota, used))) {
-            // one thread; its kept weights up to the target
-            uint32_t won = 0;
-            int at = -1;
-            auto look = [&](uint32_t w, int i) {
-                const bool in = w > theta || (w == theta && used < quota);
-                used += w == theta;
-                if (in && cur <= target) {  // (the last one that starts at or before the target)
-                    won = w;
-                    at = i;
-                    cur += w;
+        const bool mine = cur <= target && target < cur + m + theta * min(static_cast<uint64_t>(t), quota - min(quota, used));
+        const uint32_t winner = __ballot_sync(~0u, mine);
+        if (winner) {
+            // one thread of the cluster; its warp weighs its logits again, 32 at a time
+            const int who = __ffs(winner) - 1, from = __shfl_sync(~0u, base, who);
+            uint64_t run = __shfl_sync(~0u, cur, who), seen = __shfl_sync(~0u, used, who);
+            for (int i0 = 0; i0 < 4 * ch; i0 += 32) {
+                const int at = from + i0 + lane;
+                uint32_t w = i0 + lane < 4 * ch && at < p.vocab ? scale(static_cast<uint32_t>(p.logits[r * p.ld + at])) : 0;
+                if (w < least) w = 0;
+                const bool tie = w == theta && w != 0;
+                const uint32_t tied = __ballot_sync(~0u, tie);
+                if (tie && seen + __popc(tied & ((1u << lane) - 1)) >= quota) w = 0;
+                if (w < theta) w = 0;
+                uint64_t to = w;  // kept mass up to and with this one
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const uint64_t x = __shfl_up_sync(~0u, to, o);
+                    if (lane >= o) to += x;
                 }
-            };
-            each([&](int k, uint4* from) {
-                const uint4 v = *from;
-                look(v.x, base + 4 * k);
-                look(v.y, base + 4 * k + 1);
-                look(v.z, base + 4 * k + 2);
-                look(v.w, base + 4 * k + 3);
-            });
-            p.token[r] = at;
-            if (p.kept) p.kept[r] = static_cast<int32_t>(above_n + quota);
-            if (p.prob) p.prob[r] = static_cast<int32_t>(((static_cast<uint64_t>(won) << 30) + (mass >> 1)) / mass);
+                if (w != 0 && run + to - w <= target && target < run + to) {
+                    p.token[r] = at;
+                    if (p.kept) p.kept[r] = static_cast<int32_t>(above_n + quota);
+                    if (p.prob) p.prob[r] = static_cast<int32_t>(((static_cast<uint64_t>(w) << 30) + (mass >> 1)) / mass);
+                }
+                run += __shfl_sync(~0u, to, 31);
+                seen += __popc(tied);
+            }
         }
-        __syncwarp();
-        copy(r + step);   // (the warp has read its part of the row)
+        release();
         __syncthreads();  // the list has been read
     }
     cp_async_wait<0>();
