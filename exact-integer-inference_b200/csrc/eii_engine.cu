@@ -1673,6 +1673,7 @@ int eii_paged_decoder_step_device_async(eii_paged_decoder* d, const int64_t* ids
     if (n_rows == 0) return EII_OK;
     if (!ids_dev || !seq_dev || !pos_dev || !table_dev) return fail(EII_ERR_ARG, "ids_dev, seq_dev, pos_dev or table_dev is null");
     if (max_len < 1 || max_len > ROPE_POS) return fail(EII_ERR_ARG, "max_len must be in [1, %d] (got %d)", ROPE_POS, max_len);
+    TRY(check_aligned("ids_dev", ids_dev, 8));
     if (n_seq < 1 || ld_table < 1) return fail(EII_ERR_ARG, "n_seq and ld_table must be >= 1 (got %d and %lld)", n_seq, (long long)ld_table);
     if (logits_dev && (ld_logits < VOCAB || (ld_logits % 4) != 0 || (reinterpret_cast<uintptr_t>(logits_dev) & 15)))
         return fail(EII_ERR_ARG, "logits_dev must be 16-byte aligned with ld >= %d, ld %% 4 == 0", VOCAB);

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cstdint>
+
 #include "eii.h"
 
 namespace eii {
@@ -35,6 +37,12 @@ struct DeviceGuard {
         if (before >= 0) cudaSetDevice(before);
     }
 };
+
+// A device array that a kernel reads or writes element by element.
+inline int check_aligned(const char* name, const void* p, int bytes) {
+    if (reinterpret_cast<uintptr_t>(p) % bytes) return fail(EII_ERR_ARG, "%s must be %d-byte aligned", name, bytes);
+    return EII_OK;
+}
 
 // `device` exists and is sm_100 (EII_ERR_CUDA / EII_ERR_ARG otherwise); leaves the current device alone.
 int check_device(int device);

@@ -31,6 +31,7 @@ int check_pages(const eii_paged* p, const eii_pages* pg) {
     if (!pg->k_pool || !pg->v_pool || !pg->table) return fail(EII_ERR_ARG, "a pool or the page table is null");
     if ((reinterpret_cast<uintptr_t>(pg->k_pool) | reinterpret_cast<uintptr_t>(pg->v_pool)) & 15)
         return fail(EII_ERR_ARG, "the pools must be 16-byte aligned");
+    TRY(check_aligned("table", pg->table, 4));
     if (pg->n_pages < 1 || pg->n_pages > INT32_MAX)
         return fail(EII_ERR_ARG, "n_pages must be in [1, 2^31) (got %lld)", (long long)pg->n_pages);
     if (pg->n_seq < 1) return fail(EII_ERR_ARG, "n_seq must be >= 1 (got %d)", pg->n_seq);
@@ -279,6 +280,10 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
     TRY(check_shift("shift_k", shift_k));
     const uintptr_t in = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
     if (in & (in_bits / 8 - 1)) return fail(EII_ERR_ARG, "q, k and v must be aligned to their elements");
+    TRY(check_aligned("seq", seq, 4));
+    TRY(check_aligned("pos", pos, 4));
+    TRY(check_aligned("q_out", q_out, 2));
+    TRY(check_aligned("kv_out", kv_out, 4));
     DeviceGuard dg(p->device);
     CK(dg.st);
     AppendParams ap{};
@@ -317,6 +322,8 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
     if (bits_c < 2 || bits_c > 32) return fail(EII_ERR_ARG, "bits_c must be in [2, 32] (got %d)", bits_c);
     if ((reinterpret_cast<uintptr_t>(q) & 1) || (reinterpret_cast<uintptr_t>(ctx) & 3))
         return fail(EII_ERR_ARG, "q and ctx must be aligned to their elements");
+    TRY(check_aligned("seq", seq, 4));
+    TRY(check_aligned("len", len, 4));
     DeviceGuard dg(p->device);
     CK(dg.st);
     PagedAttnParams ap{};

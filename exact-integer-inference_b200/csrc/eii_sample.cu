@@ -36,11 +36,10 @@ int launch_sample(const eii_sampler* s, const SampleParams& p, int cs, cudaStrea
     return EII_OK;
 }
 
-// Once per handle: the kernel's shared memory and cluster limits on the current device.
+// Once per handle: the kernel's shared memory on the current device.
 int allow_sample() {
     CK(cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize,
                             SAMPLE_MAX_CHUNKS * 16 * SAMPLE_THREADS + static_cast<int>(sizeof(SampleShared))));
-    CK(cudaFuncSetAttribute(k_sample, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return EII_OK;
 }
 
@@ -83,9 +82,10 @@ int eii_sample(eii_sampler* s, const int32_t* logits, int64_t ld, int n_rows, in
     if (!logits || !u || !token) return fail(EII_ERR_ARG, "logits, u or token is null");
     if (vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return fail(EII_ERR_ARG, "vocab must be in [1, %d] (got %d)", SAMPLE_MAX_VOCAB, vocab);
     if (ld < vocab) return fail(EII_ERR_ARG, "ld must be >= %d (got %lld)", vocab, (long long)ld);
-    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(u)) & 3)
-        return fail(EII_ERR_ARG, "logits and u must be 4-byte aligned");
-    if (reinterpret_cast<uintptr_t>(token) & 7) return fail(EII_ERR_ARG, "token must be 8-byte aligned");
+    const struct { const char* name; const void* p; } words[] = {{"logits", logits}, {"u", u}, {"inv_temp", inv_temp}, {"top_k", top_k},
+                                                                 {"top_p", top_p}, {"min_p", min_p}, {"kept", kept}, {"prob", prob}};
+    for (const auto& w : words) TRY(check_aligned(w.name, w.p, 4));
+    TRY(check_aligned("token", token, 8));
     DeviceGuard dg(s->device);
     CK(dg.st);
     SampleParams p{};

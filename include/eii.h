@@ -299,7 +299,8 @@ void eii_paged_close(eii_paged* p);
  * valid, its logits are undefined.  pos[r] < max_len <= 512 for every row.
  * ids_dev int64, seq_dev, pos_dev, table_dev int32, logits_dev (nullable) int32 [n_rows][ld_logits] as in
  * eii_forward_device.  Like eii_decoder_step_device_async the step returns once it is enqueued
- * (null stream = the engine's), uses the engine's workspace, and leaves device-side errors to
+ * (null stream = the engine's own, which does not wait for the legacy default stream that null means to
+ * eii_sample: a loop of both passes one stream of its own), uses the engine's workspace, and leaves device-side errors to
  * eii_paged_decoder_sync, after which the rows of the failed steps have to be appended again. */
 typedef struct eii_paged_decoder eii_paged_decoder;
 int eii_paged_decoder_open(eii_engine* e, int page_size, int cache_bits, int64_t n_pages, eii_paged_decoder** out);

@@ -288,7 +288,8 @@ def test_cache_refusals(torch):
                 lambda: append(q_out_ptr=q.data_ptr()), lambda: append(q_ptr=q.data_ptr(), q_out_ptr=q.data_ptr(), shift_q=0),
                 lambda: attend(n=3), lambda: attend(max_len=131073), lambda: attend(max_len=-1), lambda: attend(prob_bits=15),
                 lambda: attend(prob_bits=20), lambda: attend(shift_s=0), lambda: attend(shift_c=63), lambda: attend(shift_c=-17), lambda: attend(bits_c=33),
-                lambda: attend(ldq=575), lambda: attend(ldc=575), lambda: c.p.pool_bytes(0)):
+                lambda: attend(seq_ptr=q.data_ptr() + 2), lambda: append(seq_ptr=q.data_ptr() + 2),
+                lambda: append(kv_out_ptr=out.data_ptr() + 2), lambda: attend(ldq=575), lambda: attend(ldc=575), lambda: c.p.pool_bytes(0)):
         with pytest.raises(_eii.EiiError) as e:
             bad()
         assert e.value.code == _eii.EII_ERR_ARG
@@ -433,6 +434,7 @@ def test_sampling_refusals(torch, sampler):
                 lambda: sampler.sample(None, 2, 64, u.data_ptr(), tok.data_ptr()),
                 lambda: sampler.sample(x.data_ptr(), 2, 64, None, tok.data_ptr()),
                 lambda: sampler.sample(x.data_ptr(), 2, 64, u.data_ptr(), None),
+                lambda: call(inv_temp_ptr=x.data_ptr() + 2), lambda: call(kept_ptr=x.data_ptr() + 1),
                 lambda: sampler.sample(x.data_ptr() + 2, 2, 64, u.data_ptr(), tok.data_ptr())):
         with pytest.raises(_eii.EiiError) as e:
             bad()
