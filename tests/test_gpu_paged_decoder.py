@@ -51,10 +51,12 @@ class Run:
         return out
 
 
-@pytest.mark.parametrize("page", [16, 64])
-def test_ragged_steps_equal_the_forward_pass(torch, eng, page):
+@pytest.mark.parametrize("page,chunk", [(16, 0), (64, 0), (32, 7)])
+def test_ragged_steps_equal_the_forward_pass(torch, eng, page, chunk, monkeypatch):
     """Prompts of different lengths in one step, a prompt in two parts, single tokens with padding between
-    them: every logits row equals the forward pass's."""
+    them, and a step in chunks of seven rows: every logits row equals the forward pass's."""
+    if chunk:
+        monkeypatch.setenv("EII_CHUNK_ROWS", str(chunk))
     rng = np.random.default_rng(page)
     lens = [5, 23, 70, 1]
     ids = [rng.integers(0, V, n) for n in lens]
