@@ -81,7 +81,7 @@ int launch_append(const AppendParams& ap, int in_bits, int num_sms, cudaStream_t
     return EII_OK;
 }
 
-constexpr int kSmemOptin = 227 * 1024 - 3072;  // dynamic shared memory of one block beside the static words
+constexpr int kSmemOptin = 224 * 1024;  // dynamic shared memory of one block beside the static words
 
 // How the work of one attention call is laid out.
 struct AttnShape {
