@@ -490,6 +490,8 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
             if (tile_i == ids_base + 16) fetch_ids();
             const int key = 32 * (first + (tile_i << stride_log2));
             uint8_t* dst = ring + at_s * C::TILE;
+            // 16-byte chunks of rows, 32 at a time; a row's chunk c lands in chunk c ^ f(row), against bank conflicts.  What
+            // depends on the lane alone is the same for every tile, the rest are constants and the halves' slots.
             const uint8_t* half[2];
             int slot[2];
 #pragma unroll
@@ -497,22 +499,21 @@ __global__ void __launch_bounds__(WARP ? 128 : BITS == 4 && HD == 64 ? 768 : 512
                 slot[h] = (key + 16 * h) & slot_mask;
                 half[h] = pool + static_cast<uint64_t>(static_cast<uint32_t>(__shfl_sync(~0u, ids, tile_i - ids_base + 16 * h))) * page_pitch;
             }
-            // 16-byte chunks of rows: chunk c of row r lands in chunk c ^ f(r), against bank conflicts
             constexpr int CH = C::ROW / 16, VCH = BITS == 4 ? CH : CH / C::SWEEPS;
+            const uint8_t* from[2] = {half[0] + slot[0] * C::ROW, half[1] + slot[1] * C::ROW};
             if (BITS == 16 && sweep_i >= 0) {
+                const int row = lane / VCH, c = lane % VCH, at = row * C::ROW + 16 * (c + VCH * sweep_i);
+                uint8_t* to = dst + row * (16 * VCH) + 16 * (c ^ 2 * (row & 3));
 #pragma unroll
-                for (int i = 0; i < VCH; ++i) {
-                    const int row = (lane + 32 * i) / VCH, c = lane % VCH, h = 32 * i >= 16 * VCH;
-                    cp_async16(dst + row * (16 * VCH) + 16 * (c ^ 2 * (row & 3)),
-                               half[h] + (slot[h] + row - 16 * h) * C::ROW + 16 * (c + VCH * sweep_i));
-                }
+                for (int i = 0; i < VCH; ++i)
+                    cp_async16(to + i * 512, from[i >= VCH / 2] + at + (i % (VCH / 2)) * (32 / VCH * C::ROW));
             } else {
+                const int row = lane / CH, c = lane % CH, at = row * C::ROW + 16 * c;
+                const int f = BITS == 16 ? (row & 1) * 4 : HD == 128 ? (row >> 1 & 1) * 2 : 0;
+                uint8_t* to = dst + row * C::ROW + 16 * (c ^ f);
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int row = (lane + 32 * i) / CH, c = lane % CH, h = 32 * i >= 16 * CH;
-                    const int f = BITS == 16 ? (row & 1) * 4 : HD == 128 ? (row >> 1 & 1) * 2 : 0;
-                    cp_async16(dst + row * C::ROW + 16 * (c ^ f), half[h] + (slot[h] + row - 16 * h) * C::ROW + 16 * c);
-                }
+                for (int i = 0; i < CH; ++i)
+                    cp_async16(to + i * 512, from[i >= CH / 2] + at + (i % (CH / 2)) * (32 / CH * C::ROW));
             }
             if (BITS == 4 && lane < 8 * A) {
                 const int h = lane >= 4 * A;
