@@ -61,8 +61,9 @@ struct SampleScale {
     // The polynomial runs on the double-precision pipe, the integer one being what bounds the kernel: u = f 2^-24
     // exactly, and y u + 2^52 rounded down is 2^52 + floor(y u) for every y below 2^30 (one rounding, at the units'
     // place).  RS(y, n) = ((2 y >> n) + 1) >> 1.
-    __device__ __forceinline__ uint32_t operator()(uint32_t logit) const {
-        const uint64_t x = static_cast<uint64_t>(row_max - logit) * b2;
+    template <bool CHECK>
+    __device__ __forceinline__ uint32_t at_distance(uint32_t d) const {
+        const uint64_t x = static_cast<uint64_t>(d) * b2;
         const uint32_t hi = static_cast<uint32_t>(x >> 32), lo = static_cast<uint32_t>(x);
         constexpr double M = 4503599627370496.0;  // 2^52
         const double u = __hiloint2double(static_cast<int>((__funnelshift_r(lo, hi, 20) & 0xFFFFFu) | 0x3FF00000u),
@@ -72,7 +73,22 @@ struct SampleScale {
         y = (M + SAMPLE_C1) - __fma_rd(y, u, M);
         const uint32_t k = static_cast<uint32_t>(__double2loint(__fma_rd(y, u, M)));
         const uint32_t w = (__funnelshift_rc((1u << 31) - 2 * k, 0, hi >> 8) + 1) >> 1;
-        return hi < (31u << 8) && logit != static_cast<uint32_t>(SAMPLE_MASKED) ? w : 0;
+        return !CHECK || hi < (31u << 8) ? w : 0;
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t logit) const {
+        return logit != static_cast<uint32_t>(SAMPLE_MASKED) ? at_distance<true>(row_max - logit) : 0;
+    }
+    // Whether at_distance<false> gives every logit's weight: from 32 octaves on the shift leaves nothing, in the
+    // 31st it leaves something for f = 0 only; so masked logits have to be 32 octaves away, and no distance may
+    // hit that place (at most one can, for b2 > 2^16).  The comparisons would be a quarter of a weight's cost.
+    __device__ bool plain() const {
+        constexpr uint64_t edge = 31ull << 40;
+        if (b2 <= 1u << 16 || static_cast<uint64_t>(row_max - static_cast<uint32_t>(SAMPLE_MASKED)) * b2 < 32ull << 40) return false;
+        const uint32_t d = static_cast<uint32_t>(static_cast<double>(edge) / b2);
+        bool hit = false;
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) hit |= static_cast<uint64_t>(d + i - 1) * b2 - edge < 1u << 16;
+        return !hit;
     }
 };
 
@@ -268,33 +284,41 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         }
         // Weights.  min-p first, whose cut is known: weights below it go.  (All three keep prefixes of one order.)
         const SampleScale scale{static_cast<uint32_t>(mx), q.b2};
-        uint64_t own_mass = 0;
-        uint32_t own_n = 0, some = 0;
         const uint32_t least = max(static_cast<uint32_t>(q.mp) << 14, 1u);
-        auto weigh_all = [&](auto with_min) {
-            each([&](int k, uint4* x) {
-                uint4 v = *x;
-                auto weigh = [&](uint32_t l) {
-                    const uint32_t w = scale(l);
-                    if (!decltype(with_min)::value) {
-                        own_n += w != 0;
-                        return w;
-                    }
-                    own_n += w >= least;
-                    return w >= least ? w : 0;
-                };
-                v = make_uint4(weigh(v.x), weigh(v.y), weigh(v.z), weigh(v.w));
-                *x = v;
-                own_mass += v.x + v.y;  // (two are at most 2^31)
-                own_mass += v.z + v.w;
-                if (k == ch >> 1) some = v.x;
-            });
+        const bool cuts_mass = q.p < 65536;
+        uint64_t own_mass = 0, mass = 0;
+        uint32_t own_n = 0, some = 0, n = p.vocab;
+
+        // The list: its length, what this thread has of it and above it, and whether it reaches up to the maximum.
+        uint32_t list_n = 0, mine_at = 0, mine_n = 0;
+        uint64_t mine_above = 0;
+        bool have_list = false, list_to_top = false, by_row = false;
+        const uint32_t* lw = cs > 1 ? sh.w + SAMPLE_LIST / 2 : sh.w;
+        const uint32_t room = cs > 1 ? SAMPLE_LIST / 2 : SAMPLE_LIST;
+        // makes the list of the mine_n words that put(place) stores for each thread
+        auto collect = [&](auto put) {
+            uint64_t none;
+            before(0, mine_n, false, none, mine_at);
+            const int now = turn;
+            if (mine_n) put(mine_at);
+            if (cs > 1) {
+                if (tid == SAMPLE_THREADS - 1) sh.block_n[now] = mine_at + mine_n;
+                cluster_barrier();
+                uint32_t to = SAMPLE_LIST / 2;
+                for (int b = 0; b < cs; ++b) {
+                    const uint32_t have = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[now], b)));
+                    for (uint32_t i = tid; i < have; i += SAMPLE_THREADS)
+                        sh.w[to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.w[i], b)));
+                    to += have;
+                }
+                list_n = to - SAMPLE_LIST / 2;
+                cluster_barrier();
+            } else {
+                if (tid == SAMPLE_THREADS - 1) sh.few_n = mine_at + mine_n;
+                __syncthreads();
+                list_n = sh.few_n;
+            }
         };
-        if (q.mp) weigh_all(std::true_type{});
-        else weigh_all(std::false_type{});
-        uint64_t mass = own_mass;
-        uint32_t n = own_n;
-        total_cluster(mass, n);
         // Once a warp needs its part of the row no more, the next row's may come.
         bool released = false;
         auto release = [&]() {
@@ -304,18 +328,123 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 released = true;
             }
         };
-        const bool cuts_n = q.k != 0 && static_cast<uint32_t>(q.k) < n, cuts_mass = q.p < 65536;
-        if (!cuts_n && !cuts_mass) release();
+
+        // A small top-k needs the weights of the highest logits only.  The distance that some more than k threads'
+        // maxima lie within is found like a guess below; all logits within it go on the list.  If k of them weigh more
+        // than a logit at that distance would, none outside can be among the k.
+        bool quick = q.k > 0 && q.k <= SAMPLE_THREADS / 2 && ch >= SAMPLE_GUESS_CHUNKS;
+        if (quick) {
+            sh.w[tid] = own_max == SAMPLE_MASKED ? ~0u : static_cast<uint32_t>(mx) - static_cast<uint32_t>(own_max);
+            __syncthreads();
+            const uint32_t want = q.k + q.k / 8 + 1;
+            uint32_t within = 0, unit = 0;  // threshold so far and what the next round adds
+#pragma unroll 1
+            for (int round = 0; round < 2; ++round) {
+                // warp b's threshold: 2^b, then one of 32 parts of the last octave
+                const uint32_t th = round == 0 ? 1u << warp : within + (warp + 1) * unit;
+                uint32_t f = 0;
+#pragma unroll
+                for (int i = lane; i < SAMPLE_THREADS / 4; i += 32) {
+                    const uint4 w = reinterpret_cast<const uint4*>(sh.w)[i];
+                    f += (w.x < th) + (w.y < th) + (w.z < th) + (w.w < th);
+                }
+                f = __reduce_add_sync(~0u, f);
+                turn ^= 1;
+                if (lane == 0) sh.warp_n[turn][warp] = f;
+                __syncthreads();
+                const uint32_t reach = __ballot_sync(~0u, sh.warp_n[turn][lane] >= want);
+                const int b = __ffs(reach) - 1;
+                if (round == 0) {
+                    if (b < 0) break;  // (too few threads have any logit near)
+                    within = b == 0 ? 0 : 1u << (b - 1);
+                    unit = max(within >> 5, 1u);
+                } else {
+                    within += (b < 0 ? 32 : b + 1) * unit;
+                }
+            }
+            if (unit == 0) within = 0;
+            if (cs > 1) {  // the first block's distance is the cluster's
+                turn ^= 1;
+                if (tid == 0) sh.block_n[turn] = within;
+                cluster_barrier();
+                within = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], 0)));
+            }
+            each([&](int, uint4* at) {
+                const uint4 v = *at;
+                own_n += (scale.row_max - v.x < within) + (scale.row_max - v.y < within) + (scale.row_max - v.z < within) +
+                         (scale.row_max - v.w < within);
+            });
+            uint32_t found = own_n;
+            total_cluster(mass, found);
+            quick = found >= static_cast<uint32_t>(q.k) && found <= room;
+            if (quick) {
+                const uint32_t outside = scale.at_distance<true>(within);
+                uint32_t sure = 0;
+                mine_n = own_n;
+                collect([&](uint32_t at) {
+                    each([&](int, uint4* from) {
+                        const uint4 v = *from;
+                        auto put = [&](uint32_t l) {
+                            if (scale.row_max - l < within) {
+                                const uint32_t w = scale(l);
+                                sure += w > outside && w >= least;
+                                sh.w[at++] = w >= least ? w : 0;
+                            }
+                        };
+                        put(v.x);
+                        put(v.y);
+                        put(v.z);
+                        put(v.w);
+                    });
+                });
+                total_cluster(mass, sure);
+                quick = sure >= static_cast<uint32_t>(q.k);
+                have_list = list_to_top = quick;
+                n = list_n;
+            }
+            if (!quick) {
+                own_n = mine_n = 0;
+                n = p.vocab;
+            }
+        }
+        if (!quick) {
+            auto weigh_all = [&](auto checked, auto counted) {
+                each([&](int k, uint4* x) {
+                    uint4 v = *x;
+                    auto weigh = [&](uint32_t l) {
+                        uint32_t w;
+                        if (decltype(checked)::value) {
+                            w = scale(l);
+                            w = w >= least ? w : 0;
+                        } else {
+                            w = scale.at_distance<false>(scale.row_max - l);
+                        }
+                        if (decltype(counted)::value) own_n += w != 0;
+                        return w;
+                    };
+                    v = make_uint4(weigh(v.x), weigh(v.y), weigh(v.z), weigh(v.w));
+                    *x = v;
+                    own_mass += v.x + v.y;  // (two are at most 2^31)
+                    own_mass += v.z + v.w;
+                    if (k == ch >> 1) some = v.x;
+                });
+            };
+            const bool need_n = q.k != 0 || !cuts_mass;
+            if (q.mp || !scale.plain()) weigh_all(std::true_type{}, std::true_type{});
+            else if (need_n) weigh_all(std::false_type{}, std::true_type{});
+            else weigh_all(std::false_type{}, std::false_type{});
+            mass = own_mass;
+            uint32_t x = own_n;
+            total_cluster(mass, x);
+            if (need_n) n = x;
+            mine_above = own_mass;
+        }
+        const bool cuts_n = quick || (q.k != 0 && static_cast<uint32_t>(q.k) < n);
+        if (quick || (!cuts_n && !cuts_mass)) release();
 
         // theta, the mass and the number of the weights above it, and how many equal to it are kept
         uint32_t theta = 0, above_n = n;
         uint64_t above = mass, quota = 0;
-        // the list: its length, what this thread has of it and above it, and whether anything is above it
-        uint32_t list_n = 0, mine_at = 0, mine_n = 0;
-        uint64_t mine_above = own_mass;
-        bool have_list = false, list_to_top = false, by_row = false;
-        const uint32_t* lw = cs > 1 ? sh.w + SAMPLE_LIST / 2 : sh.w;
-        const uint32_t room = cs > 1 ? SAMPLE_LIST / 2 : SAMPLE_LIST;
 #pragma unroll 1
         for (int stage = 0; stage < 2; ++stage) {
             const bool by_count = stage == 0;  // top-k, then top-p
@@ -361,7 +490,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 // on four blocks takes 20 us without and 25 with.)
                 uint32_t guess = 0;
                 if (c > room && ch >= SAMPLE_GUESS_CHUNKS && (!by_count || goal <= SAMPLE_THREADS / 2)) {
-                    const uint32_t top = scale(own_max);
+                    const uint32_t top = scale(static_cast<uint32_t>(own_max));
                     sh.w[tid] = by_count ? (top >= least ? top : 0) : (some + 1024) >> 11;  // (masses in units of 2^11)
                     __syncthreads();
                     const uint64_t want = by_count ? goal : (above - goal) / static_cast<uint32_t>(4 * ch * cs);
@@ -442,36 +571,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                             in_n += (v.x - lo < hi - lo) + (v.y - lo < hi - lo) + (v.z - lo < hi - lo) + (v.w - lo < hi - lo);
                         });
                     }
-                    uint64_t none;
-                    before(0, in_n, false, none, mine_at);
                     mine_n = in_n;
                     mine_above = up_mass;
-                    uint32_t at = mine_at;
-                    if (in_n)
+                    collect([&](uint32_t at) {
                         each([&](int, uint4* from) {
                             const uint4 v = *from;
-                            if (v.x - lo < hi - lo) sh.w[at++] = v.x;
-                            if (v.y - lo < hi - lo) sh.w[at++] = v.y;
-                            if (v.z - lo < hi - lo) sh.w[at++] = v.z;
-                            if (v.w - lo < hi - lo) sh.w[at++] = v.w;
+                            if (max(max(v.x, v.y), max(v.z, v.w)) < lo) return;
+                            auto put = [&](uint32_t w) {
+                                const bool in = w - lo < hi - lo;
+                                if (in) sh.w[at] = w;
+                                at += in;
+                            };
+                            put(v.x);
+                            put(v.y);
+                            put(v.z);
+                            put(v.w);
                         });
-                    if (cs > 1) {
-                        if (tid == SAMPLE_THREADS - 1) sh.block_n[turn] = at;
-                        cluster_barrier();
-                        uint32_t to = SAMPLE_LIST / 2;
-                        for (int b = 0; b < cs; ++b) {
-                            const uint32_t have = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], b)));
-                            for (uint32_t i = tid; i < have; i += SAMPLE_THREADS)
-                                sh.w[to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.w[i], b)));
-                            to += have;
-                        }
-                        list_n = to - SAMPLE_LIST / 2;
-                        cluster_barrier();
-                    } else {
-                        if (tid == SAMPLE_THREADS - 1) sh.few_n = at;
-                        __syncthreads();
-                        list_n = sh.few_n;
-                    }
+                    });
                     c = list_n;
                     have_list = true;
                     list_to_top = hi == SAMPLE_TOP;

@@ -114,18 +114,13 @@ def weights(row, inv_temp):
     """Integer weights of one row of int64 logits."""
     row = np.asarray(row, I64)
     b2 = (int(inv_temp) * LOG2E_Q24 + (1 << 15)) >> 16
-    w = np.zeros(row.size, I64)
-    top = int(row.max())
-    for i in np.flatnonzero(row != MASKED):
-        x = (top - int(row[i])) * b2
-        n, f = x >> 40, ((x >> 16) & 0xFFFFFF) << 7
-        if n > 30:
-            continue
-        y = SAMPLE_C[3]
-        for c in (SAMPLE_C[2], SAMPLE_C[1], SAMPLE_C[0], 1 << 30):
-            y = c - ((y * f) >> 31)
-        w[i] = int(rs(y, n)) if n else y
-    return w
+    x = (row.max() - row) * b2  # (below 2^32 2^31)
+    n, f = x >> 40, ((x >> 16) & 0xFFFFFF) << 7
+    y = np.full(row.size, SAMPLE_C[3], I64)
+    for c in (SAMPLE_C[2], SAMPLE_C[1], SAMPLE_C[0], 1 << 30):
+        y = c - ((y * f) >> 31)
+    s = np.minimum(n, 31)
+    return np.where((n <= 30) & (row != MASKED), (y + ((I64(1) << s) >> 1)) >> s, 0)
 
 
 def draw(row, u, inv_temp=65536, top_k=0, top_p=65536, min_p=0):
@@ -142,12 +137,9 @@ def draw(row, u, inv_temp=65536, top_k=0, top_p=65536, min_p=0):
     order = order[:int(np.searchsorted(np.cumsum(w[order]), goal)) + 1]
     mass = int(w[order].sum())
     target = int(u) * mass >> 32
-    run = 0
-    for i in np.sort(order):
-        run += int(w[i])
-        if run > target:
-            return int(i), order.size, (int(w[i]) * (1 << 30) + mass // 2) // mass
-    raise AssertionError("the target lies below the mass")
+    ids = np.sort(order)
+    i = int(ids[np.searchsorted(np.cumsum(w[ids]), target, side="right")])
+    return i, order.size, (int(w[i]) * (1 << 30) + mass // 2) // mass
 
 
 # ----------------------------------------------------------------------------- the model, 4-bit cache

@@ -424,6 +424,32 @@ def test_sampling_many_rows(torch, sampler):
     check_draw(torch, sampler, lg, words(rng, 3), top_k=np.full(3, 100000))
 
 
+@pytest.mark.parametrize("n,v,pad", [(90, 20501, 3), (80, 49152, 0), (5, 128003, 1)])
+def test_sampling_long_rows(torch, sampler, n, v, pad):
+    """Rows long enough for the searches that start from a sample (one block per row, and a cluster): every
+    kind of row beside an ordinary one, small and large top-k, cuts within ties, too few logits for top-k,
+    distances at the last octave's edge."""
+    rng = np.random.default_rng(v)
+    lg = (rng.normal(0, 2.6, (n, v)) * 65536).round().astype(np.int64)
+    lg[rng.random((n, v)) < 0.01] = osv.MASKED
+    kinds = [lambda r: np.zeros(v), lambda r: np.full(v, osv.MASKED), lambda r: np.where(rng.random(v) < 3 / v, r, osv.MASKED),
+             lambda r: rng.integers(-4, 5, v) * 20000, lambda r: rng.integers(-(1 << 31) + 1, 1 << 31, v),
+             lambda r: np.where(np.arange(v) < 40, 5 << 16, r), lambda r: r - (1 << 31) + (30 << 16),
+             lambda r: -(rng.integers(30 << 16, 32 << 16, v) * 0.6931).astype(np.int64) * (np.arange(v) > 0),
+             lambda r: np.sort(r), lambda r: np.where(np.arange(v) % 48 == 7, r + (9 << 16), r)]
+    for i in range(n):
+        if i % 2 == 0:
+            lg[i] = np.maximum(kinds[i // 2 % len(kinds)](lg[i]), osv.MASKED)
+    u = words(rng, n)
+    t = np.where(np.arange(n) % 3 == 0, 65536, (65536 / rng.uniform(.05, 3, n)).round()).astype(np.int64)
+    for k in (1, 2, 50, 300, 512, 513, 5000):
+        check_draw(torch, sampler, lg, u, pad, inv_temp=t, top_k=np.full(n, k))
+        check_draw(torch, sampler, lg, u, pad, top_k=np.full(n, k), top_p=rng.integers(0, 65537, n), min_p=rng.integers(0, 300, n))
+    for p in (100, 30000, 60000, 65000, 65530):
+        check_draw(torch, sampler, lg, u, pad, inv_temp=t, top_p=np.full(n, p))
+    check_draw(torch, sampler, lg, u, pad, inv_temp=np.where(np.arange(n) % 2, 1, 1 << 22), top_p=np.full(n, 64000))
+
+
 def test_sampling_refusals(torch, sampler):
     import _eii
     x = torch.zeros(2, 64, dtype=torch.int32, device="cuda")
