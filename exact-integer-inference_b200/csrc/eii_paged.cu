@@ -89,27 +89,33 @@ struct AttnShape {
     int warps, cs;  // warps per block, blocks per cluster
 };
 
-// Measured in captured graphs (9 query heads on 3 kv heads, head_dim 64, 4 bits unless said, us):
-//  - one warp per item once items fill the SMs and none is long: 4096 x 128 keys 56 (two warps per item 90,
-//    eight 193), at 16 bits 94 (140); 512 x 512 at 16 bits 50 (four warps 60); but 64 x 512 10.2 with eight.
-//    A warp's fixed cost is about two tiles' work.
-//  - eight warps otherwise: 64 x 512 10.2 (four 11.8); four when there are many items of at most 1024 keys.
-//  - clusters until there are eight warps per SM and as long as a warp keeps two tiles: 8 x 4096 13.7 with
-//    eight blocks (four 14.0, sixteen 25.5), 1 x 4096 11.1 (sixteen 11.7), 8 x 32768 42.6 (sixteen 53.6);
-//    two blocks more for long sequences that would leave a tail (64 x 4096 32.4, one block over 39) or whose
-//    scores (nh int16 per key) would keep a second block off the SM: 128 rows x 6000 keys of 32 heads on 8 of
-//    head_dim 128 276 with two blocks, 370 with one.
-//  - sixteen warps for the longest of a few sequences: 1 x 65521 30 (eight 36).
-AttnShape attn_shape(int64_t items, int tiles, int nh, int sms) {
-    if (tiles <= 32 && items >= 8 * sms) return {true, 4, 1};
+// Measured in captured graphs (sequences x keys, 9 query heads on 3 kv heads, head_dim 64, 4 bits unless said, us):
+//  - one warp per item once items fill the SMs and none is long: 4096 x 128 keys 58 (two warps per item 90,
+//    eight 193), at 16 bits 88 (140).  A warp's fixed cost is about two tiles' work.
+//  - otherwise as few warps per block as give eight warps per SM: 64 x 512 9.5 with eight (four 10.6), 200 x 512 17.3
+//    with two (four 19.7, eight 23.2);
+//  - for longer items blocks of four warps, of which more fit an SM, where clusters of eight reach that: 64 x 4096
+//    31.1 (eight warps 34.4), at 16 bits 46.6 (63.5), 512 x 2000 92.6 (107.5), 16 x 16384 32.0 (36.6); eight warps for
+//    fewer items and for head_dim 128: 64 x 4096 of 32 heads on 8 119 (four 146);
+//  - clusters until there are eight warps per SM, as long as a warp keeps two tiles: 8 x 4096 13.1 with eight blocks
+//    (sixteen 25.5), 8 x 32768 37 (of sixteen warps 46); and until a block's scores (nh int16 per key) leave room for a second
+//    block on the SM: 128 rows x 6000 keys of 32 heads on 8 of head_dim 128 271 with two blocks, 370 with one;
+//  - sixteen warps for the longest of a few sequences: 1 x 65521 26 (eight 36).
+AttnShape attn_shape(int64_t items, int tiles, int nh, int hd, int sms) {
+    const int64_t enough = 8 * static_cast<int64_t>(sms);
+    if (tiles <= 32 && items >= enough) return {true, 4, 1};
     int warps = 1, cs = 1;
     while (warps < 8 && warps < tiles) warps *= 2;
-    if (warps == 8 && tiles <= 32 && items >= 4 * sms) warps = 4;
+    if (tiles <= 32) {
+        while (warps > 2 && items * (warps / 2) >= enough) warps /= 2;
+    } else if (hd == 64 && items * 8 * 4 >= enough) {
+        warps = 4;
+    }
     while (cs < PATTN_MAX_CLUSTER &&
-           ((tiles + cs - 1) / cs * 32 > PATTN_MAX_PART || (items * cs * warps < 8 * sms && 4 * cs * warps <= tiles) ||
-            (cs < 4 && items * cs * warps < 16 * sms && 16 * cs * warps <= tiles) || (cs < 4 && nh * ((tiles + cs - 1) / cs) > 600)))
+           ((tiles + cs - 1) / cs * 32 > PATTN_MAX_PART || (items * cs * warps < enough && 4 * cs * warps <= tiles) ||
+            (cs < 4 && nh * ((tiles + cs - 1) / cs) > 600)))
         cs *= 2;
-    if (cs == PATTN_MAX_CLUSTER && items * cs * 16 <= 8 * sms && 4 * cs * warps <= tiles) warps = 16;
+    if (cs == PATTN_MAX_CLUSTER && items * cs * 16 <= enough && 4 * cs * warps <= tiles) warps = 16;
     return {false, warps, cs};
 }
 
@@ -119,7 +125,7 @@ int launch_attention_nh(const eii_paged* p, const PagedAttnParams& ap, cudaStrea
     const int tiles = (ap.max_len + 31) / 32 + (ap.max_len == 0);
     const int64_t items = static_cast<int64_t>(ap.n_rows) * p->n_kv * ((ap.g.group + NH - 1) / NH);
     if (items > INT32_MAX / PATTN_MAX_CLUSTER) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
-    AttnShape s = attn_shape(items, tiles, NH, p->num_sms);
+    AttnShape s = attn_shape(items, tiles, NH, HD, p->num_sms);
     if (s.warp) {
         k_paged_attention<HD, BITS, NH, true><<<static_cast<unsigned>((items + s.warps - 1) / s.warps), 32 * s.warps,
                                                C::smem_warp(s.warps, tiles * 32), st>>>(ap, 1, tiles * 32, static_cast<int>(items));

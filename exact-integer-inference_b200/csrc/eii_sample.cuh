@@ -135,8 +135,8 @@ struct SampleShared {
 };
 static_assert(SAMPLE_MAX_CHUNKS * 16 * SAMPLE_THREADS + sizeof(SampleShared) <= 227 * 1024, "shared memory");
 
-// Bound by the integer pipe: of 52,000 cycles of a row of 49152 (top-p) the weights take 17,000, each of two
-// passes 5,000, the sample 6,000, the list and its search 12,000.  4096 such rows take 911 us, 0.88 TB/s of the 6.5
+// Bound by the integer pipe: of 49,000 cycles of a row of 49152 (top-p) the weights take about 14,000, each of two
+// passes 5,000, the sample 6,000, the list and its search 12,000.  4096 such rows take 855 us, 0.94 TB/s of the 6.5
 // that a copy reaches.  The weights in registers instead of shared memory (96 per thread, 512 threads) took 1,600
 // us: unrolled code and spills.
 __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams p, const int cs, const int ch, const int aligned) {
@@ -355,9 +355,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 const uint32_t reach = __ballot_sync(~0u, sh.warp_n[turn][lane] >= want);
                 const int b = __ffs(reach) - 1;
                 if (round == 0) {
-                    if (b < 0) break;  // (too few threads have any logit near)
-                    within = b == 0 ? 0 : 1u << (b - 1);
-                    unit = max(within >> 5, 1u);
+                    // (Where too few threads have any logit near, `unit` stays 0 and the second round is gone through
+                    // all the same: `turn` has to stay one for the cluster's blocks.)
+                    within = b <= 0 ? 0 : 1u << (b - 1);
+                    if (b >= 0) unit = max(within >> 5, 1u);
                 } else {
                     within += (b < 0 ? 32 : b + 1) * unit;
                 }

@@ -450,6 +450,24 @@ def test_sampling_long_rows(torch, sampler, n, v, pad):
     check_draw(torch, sampler, lg, u, pad, inv_temp=np.where(np.arange(n) % 2, 1, 1 << 22), top_p=np.full(n, 64000))
 
 
+@pytest.mark.parametrize("n,v,near", [(2, 196609, 0), (1, 229377, 600), (40, 81925, 81925), (70, 49152, 24000), (20, 98304, 30000), (20, 98304, 77777)])
+def test_sampling_uneven_blocks(torch, sampler, n, v, near):
+    """Rows of several blocks of which some have hardly a logit: rows that end before the last block, and rows
+    masked behind (every other one: before) their first `near` logits."""
+    rng = np.random.default_rng(near + v)
+    lg = (rng.normal(0, 2.6, (n, v)) * 65536).round().astype(np.int64)
+    for i in range(n):
+        if near and i % 2:
+            lg[i, :v - near] = osv.MASKED
+        elif near:
+            lg[i, near:] = osv.MASKED
+    u = words(rng, n)
+    for k in (1, 50, 200, 500):
+        check_draw(torch, sampler, lg, u, top_k=np.full(n, k))
+        check_draw(torch, sampler, lg, u, 1, top_k=np.full(n, k), top_p=np.full(n, 60000))
+    check_draw(torch, sampler, lg, u, top_p=np.full(n, 60000))
+
+
 def test_sampling_refusals(torch, sampler):
     import _eii
     x = torch.zeros(2, 64, dtype=torch.int32, device="cuda")
