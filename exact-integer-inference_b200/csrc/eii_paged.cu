@@ -91,9 +91,12 @@ struct AttnShape {
 
 // Measured in captured graphs (sequences x keys, 9 query heads on 3 kv heads, head_dim 64, 4 bits unless said, us):
 //  - one warp per item once items fill the SMs and none is long: 4096 x 128 keys 58 (two warps per item 90,
-//    eight 193), at 16 bits 88 (140).  A warp's fixed cost is about two tiles' work.
-//  - otherwise as few warps per block as give eight warps per SM: 64 x 512 9.5 with eight (four 10.6), 200 x 512 17.3
-//    with two (four 19.7, eight 23.2);
+//    eight 193), at 16 bits 88 (140), 512 x 512 at 16 bits 46 (four 60), 400 x 1000 45.8 (four 39.9).  A warp's fixed
+//    cost is about two tiles' work.  At 16 bits and head_dim 128 the warps' rings (8 KB a tile) leave few on an SM:
+//    1000 x 64 of 32 heads on 8 96 (two warps 142), x 128 221 (194), 160 x 500 142 (99).
+//  - otherwise as few warps per block as give eight warps per SM, two at least and from 17 tiles on four: 64 x 512 9.5
+//    with eight (four 10.6), 200 x 512 17.3 with two (four 19.7, eight 23.2), 160 x 1000 of 32 heads on 8 of head_dim
+//    128 83 with four (two 100, eight 94);
 //  - for longer items blocks of four warps, of which more fit an SM, where clusters of eight reach that: 64 x 4096
 //    31.1 (eight warps 34.4), at 16 bits 46.6 (63.5), 512 x 2000 92.6 (107.5), 16 x 16384 32.0 (36.6); eight warps for
 //    fewer items and for head_dim 128: 64 x 4096 of 32 heads on 8 119 (four 146);
@@ -101,13 +104,14 @@ struct AttnShape {
 //    (sixteen 25.5), 8 x 32768 37 (of sixteen warps 46); and until a block's scores (nh int16 per key) leave room for a second
 //    block on the SM: 128 rows x 6000 keys of 32 heads on 8 of head_dim 128 271 with two blocks, 370 with one;
 //  - sixteen warps for the longest of a few sequences: 1 x 65521 26 (eight 36).
-AttnShape attn_shape(int64_t items, int tiles, int nh, int hd, int sms) {
+AttnShape attn_shape(int64_t items, int tiles, int nh, int hd, int bits, int sms) {
     const int64_t enough = 8 * static_cast<int64_t>(sms);
-    if (tiles <= 32 && items >= enough) return {true, 4, 1};
+    if (tiles <= (hd == 128 && bits == 16 ? 3 : 16) && items >= enough) return {true, 4, 1};
     int warps = 1, cs = 1;
     while (warps < 8 && warps < tiles) warps *= 2;
     if (tiles <= 32) {
-        while (warps > 2 && items * (warps / 2) >= enough) warps /= 2;
+        const int least = tiles <= 16 ? 2 : 4;
+        while (warps > least && items * (warps / 2) >= enough) warps /= 2;
     } else if (hd == 64 && items * 8 * 4 >= enough) {
         warps = 4;
     }
@@ -125,7 +129,7 @@ int launch_attention_nh(const eii_paged* p, const PagedAttnParams& ap, cudaStrea
     const int tiles = (ap.max_len + 31) / 32 + (ap.max_len == 0);
     const int64_t items = static_cast<int64_t>(ap.n_rows) * p->n_kv * ((ap.g.group + NH - 1) / NH);
     if (items > INT32_MAX / PATTN_MAX_CLUSTER) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
-    AttnShape s = attn_shape(items, tiles, NH, HD, p->num_sms);
+    AttnShape s = attn_shape(items, tiles, NH, HD, BITS, p->num_sms);
     if (s.warp) {
         k_paged_attention<HD, BITS, NH, true><<<static_cast<unsigned>((items + s.warps - 1) / s.warps), 32 * s.warps,
                                                C::smem_warp(s.warps, tiles * 32), st>>>(ap, 1, tiles * 32, static_cast<int>(items));
