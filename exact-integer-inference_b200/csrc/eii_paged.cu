@@ -103,7 +103,8 @@ struct AttnShape {
 //  - clusters until there are eight warps per SM, as long as a warp keeps two tiles: 8 x 4096 13.1 with eight blocks
 //    (sixteen 25.5), 8 x 32768 37 (of sixteen warps 46); and until a block's scores (nh int16 per key) leave room for a second
 //    block on the SM: 128 rows x 6000 keys of 32 heads on 8 of head_dim 128 271 with two blocks, 370 with one;
-//  - sixteen warps for the longest of a few sequences: 1 x 65521 26 (eight 36).
+//  - sixteen warps for the longest of a few sequences: 1 x 65521 24 (eight 27), at 16 bits 30 (35), 2 x 65521 27 (31);
+//    not with two tiles a warp: 1 x 16384 of 32 heads on 8 of head_dim 128 44 (eight 27).
 AttnShape attn_shape(int64_t items, int tiles, int nh, int hd, int bits, int sms) {
     const int64_t enough = 8 * static_cast<int64_t>(sms);
     if (tiles <= (hd == 128 && bits == 16 ? 3 : 16) && items >= enough) return {true, 4, 1};
@@ -119,15 +120,35 @@ AttnShape attn_shape(int64_t items, int tiles, int nh, int hd, int bits, int sms
            ((tiles + cs - 1) / cs * 32 > PATTN_MAX_PART || (items * cs * warps < enough && 4 * cs * warps <= tiles) ||
             (cs < 4 && nh * ((tiles + cs - 1) / cs) > 600)))
         cs *= 2;
-    if (cs == PATTN_MAX_CLUSTER && items * cs * 16 <= enough && 4 * cs * warps <= tiles) warps = 16;
+    if (cs >= 8 && items * cs <= sms && 8 * cs * warps <= tiles) warps = 16;
     return {false, warps, cs};
+}
+
+int attn_tiles(const PagedAttnParams& ap) { return ap.max_len > 0 ? (ap.max_len + 31) / 32 : 1; }
+int64_t attn_items(const PagedAttnParams& ap, int nh) {
+    return static_cast<int64_t>(ap.n_rows) * ap.g.n_kv * ((ap.g.group + nh - 1) / nh);
+}
+
+// Query heads of one item.  All that share a kv head (up to four) take its keys apart once; but where the blocks of
+// items with one or two heads leave SMs idle all the same, a block with less to do is done sooner.  Measured as above,
+// one, two and three heads: 1 x 200 keys 5.4, 6.0, 7.0 (at 16 bits 6.6, 7.0, 7.8), 16 x 512 6.4, 7.5, 8.4, 1 x 4096
+// 8.4, 9.3, 10.5; but with more blocks than SMs 8 x 4096 20.6, 14.7, 13.1; from 17 tiles on two thirds of the SMs
+// are as much as pays, as clusters have to fit: 16 x 1000 at 16 bits 14.9, 12.9, 12.1.
+int attn_heads(const PagedAttnParams& ap, int hd, int bits, int sms) {
+    const int most = ap.g.group < PATTN_MAX_HEADS ? ap.g.group : PATTN_MAX_HEADS, tiles = attn_tiles(ap);
+    for (int nh = 1; nh <= 2 && nh < most; ++nh) {
+        const AttnShape s = attn_shape(attn_items(ap, nh), tiles, nh, hd, bits, sms);
+        const int64_t blocks = attn_items(ap, nh) * s.cs;
+        if (!s.warp && (tiles <= 16 ? blocks <= sms : 3 * blocks <= 2 * sms)) return nh;
+    }
+    return most;
 }
 
 template <int HD, int BITS, int NH>
 int launch_attention_nh(const eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
     using C = PattnCfg<HD, BITS, NH>;
-    const int tiles = (ap.max_len + 31) / 32 + (ap.max_len == 0);
-    const int64_t items = static_cast<int64_t>(ap.n_rows) * p->n_kv * ((ap.g.group + NH - 1) / NH);
+    const int tiles = attn_tiles(ap);
+    const int64_t items = attn_items(ap, NH);
     if (items > INT32_MAX / PATTN_MAX_CLUSTER) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
     AttnShape s = attn_shape(items, tiles, NH, HD, BITS, p->num_sms);
     if (s.warp) {
@@ -155,7 +176,7 @@ int launch_attention_nh(const eii_paged* p, const PagedAttnParams& ap, cudaStrea
 
 template <int HD, int BITS>
 int launch_attention(const eii_paged* p, const PagedAttnParams& ap, cudaStream_t st) {
-    switch (ap.g.group) {
+    switch (attn_heads(ap, HD, BITS, p->num_sms)) {
         case 1: return launch_attention_nh<HD, BITS, 1>(p, ap, st);
         case 2: return launch_attention_nh<HD, BITS, 2>(p, ap, st);
         case 3: return launch_attention_nh<HD, BITS, 3>(p, ap, st);
@@ -173,12 +194,10 @@ int allow_attention() {
     return EII_OK;
 }
 template <int HD, int BITS>
-int allow_attention(int group) {
-    switch (group) {
-        case 1: return allow_attention<HD, BITS, 1>();
-        case 2: return allow_attention<HD, BITS, 2>();
-        case 3: return allow_attention<HD, BITS, 3>();
-    }
+int allow_attention() {
+    TRY((allow_attention<HD, BITS, 1>()));
+    TRY((allow_attention<HD, BITS, 2>()));
+    TRY((allow_attention<HD, BITS, 3>()));
     return allow_attention<HD, BITS, 4>();
 }
 
@@ -249,9 +268,8 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
             cudaMemset(p->err, 0, sizeof(int)) != cudaSuccess)
             rc = fail(EII_ERR_CUDA, "table upload failed: %s", cudaGetErrorString(cudaGetLastError()));
     }
-    const int group = n_heads / n_kv;
-    if (rc == EII_OK && head_dim == 64) rc = cache_bits == 4 ? allow_attention<64, 4>(group) : allow_attention<64, 16>(group);
-    else if (rc == EII_OK) rc = cache_bits == 4 ? allow_attention<128, 4>(group) : allow_attention<128, 16>(group);
+    if (rc == EII_OK && head_dim == 64) rc = cache_bits == 4 ? allow_attention<64, 4>() : allow_attention<64, 16>();
+    else if (rc == EII_OK) rc = cache_bits == 4 ? allow_attention<128, 4>() : allow_attention<128, 16>();
     if (rc != EII_OK) {
         cudaFree(p->mem);
         delete p;

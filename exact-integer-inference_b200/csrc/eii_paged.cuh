@@ -402,9 +402,9 @@ __device__ __forceinline__ uint32_t prob_exact(uint32_t q, uint32_t e, int pb, u
 // An item with fewer heads than NH computes the absent ones from zeros and drops them.
 // Bound by instruction latency and issue, not by memory: a tile of 32 keys and three heads is about 700 instructions
 // of its warp.  4096 sequences of 128 keys at 16 bits take 88 us (0.61 of the copy rate; 227 without the ring and
-// with four warps per item), 512 of up to 512 keys at 4 bits 27, one of 65521 at 4 bits 26.
+// with four warps per item), 512 of up to 512 keys at 4 bits 27, one of 65521 at 4 bits 24.
 // The bounds give a thread 128 registers; with room for 24 warps per SM instead of 16 (80 registers at 4 bits and
-// head_dim 64) the last two took 32 and 29.
+// head_dim 64) 512 of up to 512 keys took 32.
 template <int HD, int BITS, int NH, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 4 : 1)
     k_paged_attention(const PagedAttnParams p, const int cs, const int part_cap, const int n_items) {

@@ -200,6 +200,21 @@ def test_attention_long(torch, bits, hd, n):
     check_attention(torch, c, rng, [0], [n - 1], n, shift_s=20)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(9, 3, 64), (8, 2, 64), (14, 2, 128)])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("n", [1, 5, 20, 130, 700])
+def test_attention_shapes(torch, heads, kv, hd, bits, n):
+    """What a launch is laid out by: rows from one to many, each against length bounds from short to the longest."""
+    rng = np.random.default_rng(n + hd + bits)
+    lens = [300, 37, 1, 640]
+    c = Cache(torch, rng, heads, kv, hd, 32, bits, lens)
+    c.fill(rng, lens)
+    seq = rng.integers(-1, 4, n)
+    length = np.where(rng.random(n) < min(1, 8 / n), np.take(lens, seq), rng.integers(0, 50, n).clip(max=np.take(lens, seq)))
+    for max_len in (640, 1200, 5000, 20000, 70000, 131072):
+        check_attention(torch, c, rng, seq, length, max_len, shift_c=16)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_attention_extremes(torch, bits):
     """Saturated scores, one key that takes all the weight, equal keys, keys beyond the table's end,
