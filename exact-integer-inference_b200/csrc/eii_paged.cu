@@ -232,7 +232,7 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
             rope_cos = c.data();
             rope_sin = s.data();
         }
-        h.resize(PAGED_DMAX + 1 + 2 * n);
+        h.resize(PATTN_EXP_BYTES / 4 + 2 * n);  // (zeros behind the exp table)
     } catch (const std::bad_alloc&) {
         return fail(EII_ERR_ARG, "out of host memory for %d positions", n_pos);
     }
@@ -242,8 +242,8 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
         const int64_t one = int64_t(1) << 30;
         if (rope_cos[i] < -one || rope_cos[i] > one || rope_sin[i] < -one || rope_sin[i] > one)
             return fail(EII_ERR_ARG, "rope table entry %zu lies outside [-2^30, 2^30]", i);
-        h[PAGED_DMAX + 1 + i] = static_cast<int32_t>(rope_cos[i]);
-        h[PAGED_DMAX + 1 + n + i] = static_cast<int32_t>(rope_sin[i]);
+        h[PATTN_EXP_BYTES / 4 + i] = static_cast<int32_t>(rope_cos[i]);
+        h[PATTN_EXP_BYTES / 4 + n + i] = static_cast<int32_t>(rope_sin[i]);
     }
     TRY(check_device(device));
     DeviceGuard dg(device);
@@ -253,7 +253,7 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
     p->device = device;
     p->n_heads = n_heads; p->n_kv = n_kv; p->hd = head_dim; p->bits = cache_bits; p->n_pos = n_pos;
     while ((1 << p->page_shift) < page_size) ++p->page_shift;
-    const size_t exp_bytes = (PAGED_DMAX + 1 + 3) / 4 * 16, rope_bytes = n * 4;  // rope rows stay 16-byte aligned
+    const size_t exp_bytes = PATTN_EXP_BYTES, rope_bytes = n * 4;  // rope rows stay 16-byte aligned
     int rc = EII_OK;
     if (cudaDeviceGetAttribute(&p->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
         cudaMalloc(&p->mem, exp_bytes + 2 * rope_bytes + 16) != cudaSuccess)
@@ -263,8 +263,7 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
         p->rope_c = reinterpret_cast<int32_t*>(p->mem + exp_bytes);
         p->rope_s = reinterpret_cast<int32_t*>(p->mem + exp_bytes + rope_bytes);
         p->err = reinterpret_cast<int*>(p->mem + exp_bytes + 2 * rope_bytes);
-        if (cudaMemcpy(p->exp_tab, h.data(), (PAGED_DMAX + 1) * 4, cudaMemcpyHostToDevice) != cudaSuccess ||
-            cudaMemcpy(p->rope_c, h.data() + PAGED_DMAX + 1, 2 * rope_bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
+        if (cudaMemcpy(p->mem, h.data(), exp_bytes + 2 * rope_bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
             cudaMemset(p->err, 0, sizeof(int)) != cudaSuccess)
             rc = fail(EII_ERR_CUDA, "table upload failed: %s", cudaGetErrorString(cudaGetLastError()));
     }

@@ -36,7 +36,7 @@ struct PagedGeom {
     const int32_t* table;
     int64_t ld_table;
     int n_seq;
-    const int32_t* exp_tab;        // [PAGED_DMAX + 1], Q30
+    const int32_t* exp_tab;        // [PAGED_DMAX + 1], Q30, and zeros to a multiple of four words
     int* err;
 };
 
@@ -308,7 +308,7 @@ constexpr int PATTN_MAX_HEADS = 4;      // query heads of one item (they share a
 constexpr int PATTN_MAX_PART = 8192;    // keys of one block: 64 KB of scores
 constexpr int PATTN_MAX_WARPS = 16;     // of one block
 constexpr int PATTN_MAX_CLUSTER = 16;
-constexpr int PATTN_EXP_BYTES = (PAGED_DMAX + 2 + 3) / 4 * 16;  // one entry more: zero
+constexpr int PATTN_EXP_BYTES = (PAGED_DMAX + 2 + 3) / 4 * 16;  // one entry more at least: zeros, in g.exp_tab too
 
 template <int HD, int BITS, int NH>
 struct PattnCfg {
@@ -534,7 +534,6 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 4 : 1)
         else cp_async_commit();
     }
     cp_async_wait<S - 1>();  // the exp table
-    if (lane < 2 && warp == 0) exp_s[PAGED_DMAX + 1 + lane] = 0;
     __syncthreads();
     if (len == 0) {
         if (!skip && rank == 0)

@@ -240,6 +240,26 @@ def test_attention_extremes(torch, bits):
             check_attention(torch, c, rng, [0], [n], 150, shift_s=shift_s, q=q, shift_c=0, bits_c=32)
 
 
+def test_attention_tables_in_used_memory(torch):
+    """Keys too far from the maximum to weigh anything, and keys behind the last, with handles whose tables lie where
+    other tables have been."""
+    import _eii
+    rng = np.random.default_rng(12)
+    one = np.full((4096, 32), 1 << 30, np.int64)
+    old = [_eii.Paged(9, 3, 64, 16, 16, rope=(one, one)) for _ in range(4)]
+    for p in old:
+        p.close()
+    kept = []
+    for i in range(12):
+        lens = [150, 33, 7]
+        c = Cache(torch, rng, 9, 3, 64, 16, 16 if i % 2 else 4, lens, n_pos=64 + 96 * i)
+        c.fill(rng, lens)
+        kept.append(c)
+        for n, max_len in ((100, 600), (40, 600), (10, 5000), (1, 70000)):
+            seq = rng.integers(0, 3, n)
+            check_attention(torch, c, rng, seq, np.take(lens, seq), max_len, shift_s=12)
+
+
 def test_attention_shared_pages(torch):
     """Two sequences that share their first pages (a common prompt)."""
     rng = np.random.default_rng(8)
