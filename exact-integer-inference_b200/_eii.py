@@ -145,6 +145,41 @@ def _c(a, dt):
     return np.ascontiguousarray(a, dtype=dt)
 
 
+def _take(cell, close):
+    h, cell[0] = cell[0], None
+    if h:
+        close(h)
+
+
+class _OnEngine:
+    """A C handle that uses its engine until it is closed.  Objects are collected in any order (both at once, too,
+    when they are part of one cycle), so the engine keeps the handle itself, in a cell that both share:
+    whichever is closed first closes it, and the other finds the cell empty."""
+
+    _cell = None
+
+    def _opened(self, engine, h, close):
+        self.engine = engine
+        self._cell, self._close = [h], close
+        engine._open[id(self._cell)] = (self._cell, close)
+
+    @property
+    def h(self):
+        """The C handle, None once this or the engine is closed."""
+        return self._cell[0] if self._cell else None
+
+    def close(self):
+        if self._cell:
+            self.engine._open.pop(id(self._cell), None)
+            _take(self._cell, self._close)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Engine:
     """One engine handle on one CUDA device (owns the device weights and workspaces)."""
 
@@ -157,8 +192,13 @@ class Engine:
             check(lib().eii_open(os.fsencode(model_bin), device, ctypes.byref(h)))
         self.h = h
         self.device = device
+        self._open = {}  # the C handles that were opened on this one: id(cell) -> (cell, close), see _OnEngine
 
     def close(self):
+        """Closes what was opened on this engine (decoders, plans), then the engine."""
+        while self.h and self._open:
+            cell, close = self._open.popitem()[1]
+            _take(cell, close)
         if self.h:
             lib().eii_close(self.h)
             self.h = None
@@ -309,7 +349,7 @@ def verify_tables(model_bin):
     check(lib().eii_verify_tables(ptr(buf), buf.nbytes))
 
 
-class LinearPlan:
+class LinearPlan(_OnEngine):
     """Device-resident Model.linear with bound weights (include/eii.h, eii_linear_plan_*):
     out = SAT_bits_out(RS(a W^T m, n + f_in - f_out)) as int32 on device buffers, with optional
     per-row digests of out and of the exact int64 accumulators."""
@@ -322,8 +362,7 @@ class LinearPlan:
         h = ctypes.c_void_p()
         check(lib().eii_linear_plan_open(engine.h, ptr(W), ptr(m), ptr(n), N, K, int(bits_in), int(f_in), int(f_out),
                                          int(bits_out), ctypes.byref(h)))
-        self.h = h
-        self.engine = engine  # the engine must outlive the plan
+        self._opened(engine, h, lib().eii_linear_plan_close)
         self.N, self.K = N, K
 
     def run(self, a_ptr, M, out_ptr, ld=None, dig_out_ptr=None, dig_acc_ptr=None, stream=None):
@@ -331,39 +370,16 @@ class LinearPlan:
         check(lib().eii_linear_plan_run(self.h, ctypes.c_void_p(a_ptr), int(M), ctypes.c_void_p(out_ptr),
                                         int(ld or self.N), v(dig_out_ptr), v(dig_acc_ptr), v(stream)))
 
-    def close(self):
-        if self.h:
-            lib().eii_linear_plan_close(self.h)
-            self.h = None
 
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
-
-
-class Decoder:
+class Decoder(_OnEngine):
     """Incremental decoding with a K/V cache (include/eii.h, eii_decoder_*), bit-exact with
     recomputation: step t returns row t of Engine.forward on the first t + 1 tokens."""
 
     def __init__(self, engine, n_seq, max_T):
         h = ctypes.c_void_p()
         check(lib().eii_decoder_open(engine.h, int(n_seq), int(max_T), ctypes.byref(h)))
-        self.h = h
-        self.engine = engine  # the engine must outlive the decoder
+        self._opened(engine, h, lib().eii_decoder_close)
         self.n_seq = int(n_seq)
-
-    def close(self):
-        if self.h:
-            lib().eii_decoder_close(self.h)
-            self.h = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
 
     @property
     def position(self):
@@ -476,26 +492,13 @@ class Paged:
         check(lib().eii_paged_sync(self.h, stream))
 
 
-class PagedDecoder:
+class PagedDecoder(_OnEngine):
     """Ragged decoding of the model on a paged cache of 16 or 4 bits (include/eii.h, eii_paged_decoder_*)."""
 
     def __init__(self, engine, page_size, cache_bits, n_pages):
-        self.h = None
         h = ctypes.c_void_p()
         check(lib().eii_paged_decoder_open(engine.h, int(page_size), int(cache_bits), int(n_pages), ctypes.byref(h)))
-        self.h = h
-        self.engine = engine  # the engine must outlive the decoder
-
-    def close(self):
-        if self.h:
-            lib().eii_paged_decoder_close(self.h)
-            self.h = None
-
-    def __del__(self):
-        try:
-            self.close()
-        except Exception:
-            pass
+        self._opened(engine, h, lib().eii_paged_decoder_close)
 
     def step_device_async(self, ids_ptr, seq_ptr, pos_ptr, n_rows, table_ptr, ld_table, n_seq, max_len, logits_ptr=None,
                           ld=VOCAB, stream=None):

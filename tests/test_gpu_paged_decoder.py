@@ -152,3 +152,21 @@ def test_paged_decoder_refusals(torch, eng):
     assert np.array_equal(run.step(ids, [0, 1], [0, 0]).cpu().numpy(), want)
     run.d.step_device_async(None, None, None, 0, None, 1, 1, 1)
     run.d.sync()
+
+
+def test_engine_closed_before_its_decoders(torch, base_model_path):
+    """Decoders that are still open, a step on its way among them, when their engine is closed: they are closed with
+    it, refuse further calls, and the next engine works."""
+    import _eii
+    for _ in range(2):
+        e = _eii.Engine(base_model_path, 0)
+        run, dense = Run(torch, e, 16, 4, 2, 32), _eii.Decoder(e, 2, 8)
+        run.step([5, 6], [0, 1], [0, 0], sync=False)
+        dense.prefill(np.array([[5], [6]]))
+        e.close()
+        assert not run.d.h and not dense.h
+        for call in (lambda: run.d.sync(), lambda: dense.step([1, 2]), lambda: run.step([5, 6], [0, 1], [1, 1])):
+            with pytest.raises(_eii.EiiError, match="decoder is null"):
+                call()
+        run.d.close()
+        dense.close()
