@@ -119,8 +119,15 @@ constexpr int SAMPLE_GUESS_CHUNKS = 6;
 constexpr int SAMPLE_LIST = 8192, SAMPLE_FEW = 64;
 constexpr uint32_t SAMPLE_TOP = (1u << 30) + 1;  // above every weight
 
-// Words that the threads of a block (and the blocks of a cluster) exchange come in two sets that take turns,
-// so that one is not overwritten before its slowest reader has it: a barrier lies between the uses of a set.
+// Words that are exchanged come in two sets that take turns, so that one is not overwritten before its slowest
+// reader has it: between two uses of a set lies another exchange, whose barrier the reader reaches after
+// its reads.  The words of a block's threads (warp_*) and those of a cluster's blocks (block_*) take turns apart: a
+// block barrier does not hold back the other blocks, so an exchange within a block must not turn the cluster's sets.
+struct SampleTurns {
+    int block = 0, cluster = 0;
+    __host__ __device__ __forceinline__ int next_block() { return block ^= 1; }
+    __host__ __device__ __forceinline__ int next_cluster() { return cluster ^= 1; }
+};
 struct SampleShared {
     uint32_t w[SAMPLE_LIST];  // the list; of a cluster's blocks the first half, the second for all
     uint32_t few[SAMPLE_FEW];
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
     // neighbours read from eight banks.
     int start = ch & 1 ? 0 : lane & 7;
     while (start >= ch) start -= ch;
-    int turn = 0;
+    SampleTurns turns;
 
     // f(number of a chunk, the chunk) over this thread's chunks
     auto each = [&](auto f) {
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
     };
     // sums over the threads of the block's first `warps` warps, in every thread
     auto total = [&](uint64_t& m, uint32_t& n, int warps) {
-        turn ^= 1;
+        const int turn = turns.next_block();
         if (warp < warps) {
             m = warp_sum47(m);
             n = __reduce_add_sync(~0u, n);
@@ -205,6 +212,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
     auto total_cluster = [&](uint64_t& m, uint32_t& n) {
         total(m, n, SAMPLE_WARPS);
         if (cs > 1) {
+            const int turn = turns.next_cluster();
             if (tid == 0) {
                 sh.block_mass[turn] = m;
                 sh.block_n[turn] = n;
@@ -227,7 +235,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                 sn += y;
             }
         }
-        turn ^= 1;
+        const int turn = turns.next_block();
         if (lane == 31) {
             sh.warp_mass[turn][warp] = sm;
             sh.warp_n[turn][warp] = sn;
@@ -240,13 +248,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         if (blocks) {
             const uint64_t bm = warp_sum47(pm);
             const uint32_t bn = __reduce_add_sync(~0u, pn);
+            const int at = turns.next_cluster();
             if (tid == 0) {
-                sh.block_mass[turn] = bm;
-                sh.block_n[turn] = bn;
+                sh.block_mass[at] = bm;
+                sh.block_n[at] = bn;
             }
             cluster_barrier();
-            M += warp_sum47(lane < rank ? static_cast<uint64_t>(ld_remote64(remote_smem(&sh.block_mass[turn], lane))) : 0);
-            N += __reduce_add_sync(~0u, lane < rank ? static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], lane))) : 0);
+            M += warp_sum47(lane < rank ? static_cast<uint64_t>(ld_remote64(remote_smem(&sh.block_mass[at], lane))) : 0);
+            N += __reduce_add_sync(~0u, lane < rank ? static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[at], lane))) : 0);
         }
     };
 
@@ -262,12 +271,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
             mx = max(mx, max(max(v.x, v.y), max(v.z, v.w)));
         });
         const int32_t own_max = mx;
-        turn ^= 1;
+        const int now = turns.next_block();
         mx = __reduce_max_sync(~0u, mx);
-        if (lane == 0) sh.warp_max[turn][warp] = mx;
+        if (lane == 0) sh.warp_max[now][warp] = mx;
         __syncthreads();
-        mx = __reduce_max_sync(~0u, sh.warp_max[turn][lane]);
+        mx = __reduce_max_sync(~0u, sh.warp_max[now][lane]);
         if (cs > 1) {
+            const int turn = turns.next_cluster();
             if (tid == 0) sh.block_max[turn] = mx;
             cluster_barrier();
             mx = __reduce_max_sync(~0u, lane < cs ? ld_remote32(remote_smem(&sh.block_max[turn], lane)) : SAMPLE_MASKED);
@@ -299,14 +309,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
         auto collect = [&](auto put) {
             uint64_t none;
             before(0, mine_n, false, none, mine_at);
-            const int now = turn;
             if (mine_n) put(mine_at);
             if (cs > 1) {
-                if (tid == SAMPLE_THREADS - 1) sh.block_n[now] = mine_at + mine_n;
+                const int turn = turns.next_cluster();
+                if (tid == SAMPLE_THREADS - 1) sh.block_n[turn] = mine_at + mine_n;
                 cluster_barrier();
                 uint32_t to = SAMPLE_LIST / 2;
                 for (int b = 0; b < cs; ++b) {
-                    const uint32_t have = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[now], b)));
+                    const uint32_t have = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], b)));
                     for (uint32_t i = tid; i < have; i += SAMPLE_THREADS)
                         sh.w[to + i] = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.w[i], b)));
                     to += have;
@@ -351,14 +361,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                     f += (w.x < th) + (w.y < th) + (w.z < th) + (w.w < th);
                 }
                 f = __reduce_add_sync(~0u, f);
-                turn ^= 1;
+                const int turn = turns.next_block();
                 if (lane == 0) sh.warp_n[turn][warp] = f;
                 __syncthreads();
                 const uint32_t reach = __ballot_sync(~0u, sh.warp_n[turn][lane] >= want);
                 const int b = __ffs(reach) - 1;
                 if (round == 0) {
-                    // (Where too few threads have any logit near, `unit` stays 0 and the second round is gone through
-                    // all the same: `turn` has to stay one for the cluster's blocks.)
+                    // (Where too few threads have any logit near, `unit` stays 0: the second round finds nothing then.)
                     within = b <= 0 ? 0 : 1u << (b - 1);
                     if (b >= 0) unit = max(within >> 5, 1u);
                 } else {
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
             }
             if (unit == 0) within = 0;
             if (cs > 1) {  // the first block's distance is the cluster's
-                turn ^= 1;
+                const int turn = turns.next_cluster();
                 if (tid == 0) sh.block_n[turn] = within;
                 cluster_barrier();
                 within = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], 0)));
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                             else f += (w.x < th11 ? w.x : 0) + (w.y < th11 ? w.y : 0) + (w.z < th11 ? w.z : 0) + (w.w < th11 ? w.w : 0);
                         }
                         f = __reduce_add_sync(~0u, f);
-                        turn ^= 1;
+                        const int turn = turns.next_block();
                         if (lane == 0) sh.warp_n[turn][warp] = f;
                         __syncthreads();
                         f = sh.warp_n[turn][lane];
@@ -521,7 +530,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams
                         if (by_count && b < 0) guess = 0;  // (fewer threads than that have any weight)
                     }
                     if (cs > 1) {  // the first block's guess is the cluster's
-                        turn ^= 1;
+                        const int turn = turns.next_cluster();
                         if (tid == 0) sh.block_n[turn] = guess;
                         cluster_barrier();
                         guess = static_cast<uint32_t>(ld_remote32(remote_smem(&sh.block_n[turn], 0)));

@@ -591,3 +591,25 @@ def test_streams_and_graphs(torch, sampler):
         assert np.array_equal(ctx.cpu().numpy().reshape(n, 9, 64), wc)
         assert tok.tolist() == [osv.draw(wc[r].reshape(-1), w[r])[0] for r in range(n)]
     sampler.sync(st(torch))
+
+
+@pytest.mark.parametrize("n,v", [(1, 49152), (3, 20000), (30, 128003), (2, 262144)])
+def test_sampling_small_top_k_over_blocks_repeated(torch, sampler, n, v):
+    """Rows on several blocks with a small top-k whose list takes an odd or an even number of steps, many calls back
+    to back: every call gives the first one's tokens, which are the oracle's."""
+    rng = np.random.default_rng(v)
+    lg = (rng.normal(0, 2.6, (n, v)) * 65536).round().astype(np.int64)
+    u = words(rng, n)
+    dl = torch.from_numpy(lg.astype(np.int32)).cuda()
+    du = torch.from_numpy(u.astype(np.uint32).view(np.int32)).cuda()
+    for k in (1, 40, 60, 90, 130, 200, 300, 400, 512):
+        dk = torch.full((n,), k, dtype=torch.int32, device="cuda")
+        tok = torch.full((200, n), -9, dtype=torch.int64, device="cuda")
+        kept = torch.full((200, n), -9, dtype=torch.int32, device="cuda")
+        for i in range(200):
+            sampler.sample(dl.data_ptr(), n, v, du.data_ptr(), tok[i].data_ptr(), top_k_ptr=dk.data_ptr(),
+                           kept_ptr=kept[i].data_ptr(), stream=st(torch))
+        sampler.sync(st(torch))
+        want = [osv.draw(lg[r], u[r], top_k=k) for r in range(n)]
+        assert tok[0].tolist() == [w[0] for w in want] and kept[0].tolist() == [w[1] for w in want]
+        assert (tok == tok[0]).all() and (kept == kept[0]).all()
