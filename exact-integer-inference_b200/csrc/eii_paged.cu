@@ -263,8 +263,10 @@ int eii_paged_open(int device, int n_heads, int n_kv, int head_dim, int page_siz
         p->rope_c = reinterpret_cast<int32_t*>(p->mem + exp_bytes);
         p->rope_s = reinterpret_cast<int32_t*>(p->mem + exp_bytes + rope_bytes);
         p->err = reinterpret_cast<int*>(p->mem + exp_bytes + 2 * rope_bytes);
+        // (a copy from pageable memory and a memset may return before they are done, and a stream that does not wait
+        // for the default stream may have the first call)
         if (cudaMemcpy(p->mem, h.data(), exp_bytes + 2 * rope_bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
-            cudaMemset(p->err, 0, sizeof(int)) != cudaSuccess)
+            cudaMemset(p->err, 0, sizeof(int)) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess)
             rc = fail(EII_ERR_CUDA, "table upload failed: %s", cudaGetErrorString(cudaGetLastError()));
     }
     if (rc == EII_OK && head_dim == 64) rc = cache_bits == 4 ? allow_attention<64, 4>() : allow_attention<64, 16>();

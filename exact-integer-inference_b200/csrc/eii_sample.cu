@@ -57,7 +57,8 @@ int eii_sampler_open(int device, eii_sampler** out) {
     if (!s) return fail(EII_ERR_ARG, "out of host memory");
     s->device = device;
     if (cudaDeviceGetAttribute(&s->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-        cudaMalloc(&s->err, 16) != cudaSuccess || cudaMemset(s->err, 0, 16) != cudaSuccess) {
+        cudaMalloc(&s->err, 16) != cudaSuccess || cudaMemset(s->err, 0, 16) != cudaSuccess ||
+        cudaStreamSynchronize(nullptr) != cudaSuccess) {  // (a memset may return before it is done)
         const int rc = fail(EII_ERR_CUDA, "sampler set-up failed: %s", cudaGetErrorString(cudaGetLastError()));
         cudaFree(s->err);
         delete s;

@@ -613,3 +613,37 @@ def test_sampling_small_top_k_over_blocks_repeated(torch, sampler, n, v):
         want = [osv.draw(lg[r], u[r], top_k=k) for r in range(n)]
         assert tok[0].tolist() == [w[0] for w in want] and kept[0].tolist() == [w[1] for w in want]
         assert (tok == tok[0]).all() and (kept == kept[0]).all()
+
+
+def test_first_call_on_a_stream_of_its_own(torch):
+    """New handles whose first call goes to a stream that does not wait for the default one: tables and error words
+    are there when the handle is."""
+    import _eii
+    rng = np.random.default_rng(21)
+    lens = [40, 9]
+    side = torch.cuda.Stream()
+    par = torch.tensor([65536, -1], dtype=torch.int32, device="cuda")
+    x = torch.zeros(2, 64, dtype=torch.int32, device="cuda")
+    u = torch.zeros(2, dtype=torch.int32, device="cuda")
+    tok = torch.zeros(2, dtype=torch.int64, device="cuda")
+    a = [rng.integers(-32768, 32768, (2, h, 64)) for h in (9, 3, 3)]
+    for i in range(10):
+        c = Cache(torch, rng, 9, 3, 64, 16, 16, lens, n_pos=20000)
+        d = [torch.from_numpy(y.astype(np.int16)).cuda() for y in a]
+        pos = np.array([39, 8], np.int32)
+        dpos = torch.from_numpy(pos).cuda()
+        torch.cuda.synchronize()
+        c.p.close()
+        c.p = _eii.Paged(9, 3, 64, 16, 16, rope=c.rope)
+        c.p.append(c.pages, d[1].data_ptr(), d[2].data_ptr(), 2, dpos.data_ptr(), 30, q_ptr=d[0].data_ptr(),
+                   q_out_ptr=d[0].data_ptr(), shift_q=30, stream=side.cuda_stream)
+        s = _eii.Sampler(0)
+        s.sample(x.data_ptr(), 2, 64, u.data_ptr(), tok.data_ptr(), top_p_ptr=par.data_ptr(), stream=side.cuda_stream)
+        c.p.sync(side.cuda_stream)
+        with pytest.raises(_eii.EiiError, match="parameter"):
+            s.sync(side.cuda_stream)
+        s.close()
+        wq = np.zeros((2, 9, 64), np.int64)
+        osv.append(*a, np.arange(2), pos, c.table, c.k, c.v, c.rope, 30, 30, wq, np.zeros((2, 2, 3, 64), np.int64))
+        assert np.array_equal(d[0].cpu().numpy(), wq)
+        c.check_pools()
