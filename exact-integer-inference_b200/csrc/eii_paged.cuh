@@ -146,6 +146,8 @@ __global__ void __launch_bounds__(256) k_paged_append(const AppendParams p, cons
         return;
     }
     const int page_id = g.table[seq * g.ld_table + (pos >> g.page_shift)];
+    // (q's loads and rotation need not wait for it; n_pages is below 2^31)
+    auto in_pool = [&]() { return static_cast<uint32_t>(page_id) < static_cast<uint32_t>(g.n_pages); };
     const int4 c4 = *reinterpret_cast<const int4*>(p.rope_c + static_cast<int64_t>(pos) * HALF + 4 * l);
     const int4 s4 = *reinterpret_cast<const int4*>(p.rope_s + static_cast<int64_t>(pos) * HALF + 4 * l);
     const int32_t cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
@@ -206,10 +208,10 @@ __global__ void __launch_bounds__(256) k_paged_append(const AppendParams p, cons
         int32_t x[8];
         const bool good = load8(static_cast<const T*>(p.q) + r * p.ldq + from * HD, x);
         rotate8(x, p.shift_q);
-        if (good && head < g.n_heads) store8(p.q_out + r * p.ldqo + head * HD, x, vec_out & 1);
+        if (good && head < g.n_heads && in_pool()) store8(p.q_out + r * p.ldqo + head * HD, x, vec_out & 1);
     }
     if (step >= steps_q + 2 * steps_kv) return;
-    if (page_id < 0 || page_id >= g.n_pages) {
+    if (!in_pool()) {
         if (lane == 0) atomicCAS(g.err, 0, ERR_PAGED_PAGE);
         return;
     }

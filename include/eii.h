@@ -231,7 +231,9 @@ int eii_linear_noalloc(const int64_t* a_dev, int M, int K, int bits_in, const in
  * run at the same time on several streams as long as their outputs do not overlap.  The caller's
  * current device is left as it was.  Argument errors are returned at once; device-side errors (an
  * index outside its range) are kept in the handle until the next eii_paged_sync, and the row concerned
- * is skipped or, with a page index out of range, has an undefined context row.
+ * is skipped: all its outputs are left as they were.  Two errors are found later than that: a page index out of
+ * range makes the row's context undefined, and an int32 q, k or v value outside int16 skips only the heads that
+ * hold one (the row's other heads are written; the row has to be appended again).
  *
  * A pool is [n_pages][n_kv] slabs of page_size positions.  16 bits: int16 [page_size][head_dim].
  * 4 bits: uint8 [page_size][head_dim / 2], then uint32 [page_size][head_dim / 64]; each group of 64

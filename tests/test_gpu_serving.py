@@ -647,3 +647,59 @@ def test_first_call_on_a_stream_of_its_own(torch):
         osv.append(*a, np.arange(2), pos, c.table, c.k, c.v, c.rope, 30, 30, wq, np.zeros((2, 2, 3, 64), np.int64))
         assert np.array_equal(d[0].cpu().numpy(), wq)
         c.check_pools()
+
+
+@pytest.mark.parametrize("heads,kv,hd,bits,n", [(9, 3, 64, 16, 3), (9, 3, 64, 4, 3), (6, 2, 128, 4, 3), (9, 3, 64, 4, 9000), (6, 2, 128, 16, 9000)])
+@pytest.mark.parametrize("what", ["seq", "pos", "page", "value"])
+def test_append_leaves_what_it_refuses(torch, heads, kv, hd, bits, n, what):
+    """A refused row leaves its q_out, its kv_out and the pools as they were; with a value outside int16 only the heads
+    that hold one do.  The other rows are appended.  Few rows (warps share a row) and many."""
+    import _eii
+    rng = np.random.default_rng(n + hd)
+    lens = [512] * (-(-n // 512) + 1)
+    c = Cache(torch, rng, heads, kv, hd, 16, bits, lens)
+    seq, pos = (np.arange(n) // 512).astype(np.int32), (np.arange(n) % 512).astype(np.int32)
+    x = [rng.normal(0, 6000, (n, h, hd)).round().clip(-32768, 32767).astype(np.int64) for h in (heads, kv, kv)]
+    bad = n // 2
+    dseq, dpos, table = seq.copy(), pos.copy(), c.table.copy()
+    heads_left = [range(heads), range(kv), range(kv)]
+    if what == "seq":
+        dseq[bad] = len(lens)
+    elif what == "pos":
+        dpos[bad] = 512
+    elif what == "page":  # (a page of its own: the others' rows lie elsewhere)
+        dseq[bad], dpos[bad] = len(lens) - 1, 40
+        table[len(lens) - 1, 40 // 16] = c.n_pages
+    else:
+        heads_left = [[heads - 1], [0], [kv - 1]]
+        for a, h, value in zip(x, (heads - 1, 0, kv - 1), (32768, -32769, 1 << 30)):
+            a[bad, h, 5] = value
+    c.dtable.copy_(torch.from_numpy(table))
+    d = [torch.from_numpy(a.astype(np.int32)).cuda() for a in x]
+    q_out = torch.full((n, heads, hd), 99, dtype=torch.int16, device="cuda")
+    kv_out = torch.full((n, 2, kv, hd), 98, dtype=torch.int32, device="cuda")
+    ds, dp = torch.from_numpy(dseq).cuda(), torch.from_numpy(dpos).cuda()
+    before = [h.copy() for h in c.host]
+    c.p.append(c.pages, d[1].data_ptr(), d[2].data_ptr(), n, dp.data_ptr(), 30, seq_ptr=ds.data_ptr(), q_ptr=d[0].data_ptr(),
+               q_out_ptr=q_out.data_ptr(), shift_q=30, in_bits=32, kv_out_ptr=kv_out.data_ptr(), stream=st(torch))
+    text = {"seq": "sequence", "pos": "position", "page": "page", "value": "int16"}[what]
+    with pytest.raises(_eii.EiiError, match=text):
+        c.p.sync(st(torch))
+    c.p.sync(st(torch))
+    wq, wkv = np.full((n, heads, hd), 99, np.int64), np.full((n, 2, kv, hd), 98, np.int64)
+    x = [a.clip(-32768, 32767) for a in x]  # (what stands there instead is put back below)
+    if what != "value":
+        seq[bad] = -1
+    osv.append(*x, seq, pos, c.table, c.k, c.v, c.rope, 30, 30, wq, wkv)
+    if what == "value":
+        wq[bad, heads - 1] = 99
+        for i, (pool, old) in enumerate(((c.k, before[0]), (c.v, before[1]))):
+            h = heads_left[1 + i][0]
+            wkv[bad, i, h] = 98
+            page, slot = int(c.table[seq[bad], pos[bad] // 16]), int(pos[bad] % 16)
+            was = osv.Pool(old, kv, hd, 16, bits)
+            for at, size in ((slot * pool.row, pool.row), (16 * pool.row + slot * hd // 16, hd // 16 if bits == 4 else 0)):
+                pool.data[page, h, at:at + size] = was.data[page, h, at:at + size]
+    assert np.array_equal(q_out.cpu().numpy(), wq)
+    assert np.array_equal(kv_out.cpu().numpy(), wkv)
+    c.check_pools()
