@@ -1704,11 +1704,14 @@ int eii_paged_decoder_sync(eii_paged_decoder* d, void* stream) {
     if (!d) return fail(EII_ERR_ARG, "decoder is null");
     CK(cudaSetDevice(d->e->device));
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : d->e->stream;
-    const int rc = eii_paged_sync(d->cache, st), rc2 = check_device_error(d->e, st);
-    // (a bad index first: the rows it leaves undefined can make later kernels report more)
-    if (rc != EII_OK && rc2 == EII_OK) return rc;
-    if (rc != EII_OK) return fail(rc, "a sequence index, position, length or page of the step lies outside its range");
-    return rc2;
+    // Both words are read and cleared.  A wait that ran out comes before an index outside its range, that before a
+    // token id; the message is that of the error returned.
+    const int rc_engine = check_device_error(d->e, st);
+    char text[1024];
+    snprintf(text, sizeof(text), "%s", g_err.c_str());
+    const int rc = eii_paged_sync(d->cache, st);
+    if (rc_engine != EII_OK && (rc == EII_OK || rc_engine != EII_ERR_ARG)) return fail(rc_engine, "%s", text);
+    return rc;
 }
 
 void eii_paged_decoder_close(eii_paged_decoder* d) {

@@ -170,3 +170,18 @@ def test_engine_closed_before_its_decoders(torch, base_model_path):
                 call()
         run.d.close()
         dense.close()
+
+
+def test_sync_names_the_error_it_returns(torch, eng):
+    """A step with a bad token id and a bad index reports the index, in its own words, and clears both; a bad token id
+    alone is reported as such."""
+    import _eii
+    run = Run(torch, eng, 16, 16, 2, 32)
+    for seq, pos, text in (([0, 2], [0, 0], "not below n_seq"), ([0, 1], [0, 32], "position lies outside"),
+                           ([0, 1], [0, 0], "token id")):
+        with pytest.raises(_eii.EiiError, match=text) as e:
+            run.step([V, 6], seq, pos)
+        assert e.value.code == _eii.EII_ERR_ARG
+        run.d.sync()
+    want = eng.forward(np.array([[5], [6]]))["logits"][:, 0]
+    assert np.array_equal(run.step([5, 6], [0, 1], [0, 0]).cpu().numpy(), want)
