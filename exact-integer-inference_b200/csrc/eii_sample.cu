@@ -78,7 +78,8 @@ int eii_sample(eii_sampler* s, const int32_t* logits, int64_t ld, int n_rows, in
                const int32_t* top_k, const int32_t* top_p, const int32_t* min_p, const uint32_t* u, int64_t* token,
                int32_t* kept, int32_t* prob, void* stream) {
     if (!s) return fail(EII_ERR_ARG, "sampler is null");
-    if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
+    // (a block's next row, the grid's width further on, has to be an int)
+    if (n_rows < 0 || n_rows > SAMPLE_MAX_ROWS) return fail(EII_ERR_ARG, "n_rows must be in [0, %d] (got %d)", SAMPLE_MAX_ROWS, n_rows);
     if (n_rows == 0) return EII_OK;
     if (!logits || !u || !token) return fail(EII_ERR_ARG, "logits, u or token is null");
     if (vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return fail(EII_ERR_ARG, "vocab must be in [1, %d] (got %d)", SAMPLE_MAX_VOCAB, vocab);
@@ -95,7 +96,7 @@ int eii_sample(eii_sampler* s, const int32_t* logits, int64_t ld, int n_rows, in
     // Blocks per row: as many as its weights need, and up to four while that leaves no row waiting (one row of
     // 49152: 38 us on one block, 24 on two, 20 on four, 21 on eight).
     int cs = 1;
-    while (cs * SAMPLE_MAX_CHUNKS * 4 * SAMPLE_THREADS < vocab || (cs < 4 && 2 * cs * n_rows <= s->num_sms && cs * 4 * SAMPLE_THREADS < vocab))
+    while (cs * SAMPLE_MAX_CHUNKS * 4 * SAMPLE_THREADS < vocab || (cs < 4 && n_rows <= s->num_sms / (2 * cs) && cs * 4 * SAMPLE_THREADS < vocab))
         cs *= 2;
     return launch_sample(s, p, cs, static_cast<cudaStream_t>(stream));
 }

@@ -23,6 +23,7 @@ constexpr int64_t SAMPLE_LOG2E_Q24 = 24204406;
 constexpr int32_t SAMPLE_MASKED = INT32_MIN;
 constexpr int SAMPLE_MAX_VOCAB = 262144;  // 2^30 x 2^18 weights: sums stay below 2^48
 constexpr int32_t SAMPLE_MAX_INV_TEMP = 1 << 22;
+constexpr int SAMPLE_MAX_ROWS = 1 << 30;
 
 enum : int { ERR_SAMPLE_PARAM = 311 };
 

@@ -323,7 +323,7 @@ void eii_paged_decoder_close(eii_paged_decoder* d); /* before its engine */
  * Per-row parameters on the device, null = off: inv_temp 1/T in Q16, [1, 2^22] (null: T = 1), top_k
  * >= 0 (0: off), top_p and min_p in Q16, [0, 65536] (65536 / 0: off).  top_k = 1 is the greedy choice.
  * u uint32 [n_rows].  Outputs: token int64 [n_rows]; nullable kept int32 (tokens kept) and prob int32
- * (Q30 probability of the token among the kept, rounded to nearest).  vocab in [1, 262144].
+ * (Q30 probability of the token among the kept, rounded to nearest).  vocab in [1, 262144], n_rows up to 2^30.
  * A parameter outside its range gives -1 and an error at eii_sampler_sync.  Enqueues on `stream`
  * (null = the legacy default stream) and returns; allocates nothing and can be captured. */
 typedef struct eii_sampler eii_sampler;

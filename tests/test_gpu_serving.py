@@ -703,3 +703,13 @@ def test_append_leaves_what_it_refuses(torch, heads, kv, hd, bits, n, what):
     assert np.array_equal(q_out.cpu().numpy(), wq)
     assert np.array_equal(kv_out.cpu().numpy(), wkv)
     c.check_pools()
+
+
+@pytest.mark.parametrize("n", [(1 << 30) + 1, (1 << 31) - 1])
+def test_sampling_refuses_rows_that_an_int_cannot_step_over(torch, sampler, n):
+    import _eii
+    x = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(_eii.EiiError, match="n_rows") as e:
+        sampler.sample(x.data_ptr(), n, 1, x.data_ptr(), x.data_ptr(), stream=st(torch))
+    assert e.value.code == _eii.EII_ERR_ARG
+    sampler.sync(st(torch))
