@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 4 : 1)
     const int ht = item % head_tiles, kv = item / head_tiles % g.n_kv, r = item / head_tiles / g.n_kv;
     const int head0 = kv * g.group + ht * NH, nh = min(NH, g.group - ht * NH);
     const int seq = p.seq ? p.seq[r] : r;
-    int len = max(p.len[r] + p.len_add, 0);
+    int len = max(min(p.len[r], INT32_MAX - 1) + p.len_add, 0);
     // a padding row, or one that is refused: all threads of the item agree
     bool skip = seq < 0 || (WARP && index >= n_items);
     if (!skip && (seq >= g.n_seq || len > p.max_len ||

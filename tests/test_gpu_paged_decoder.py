@@ -185,3 +185,16 @@ def test_sync_names_the_error_it_returns(torch, eng):
         run.d.sync()
     want = eng.forward(np.array([[5], [6]]))["logits"][:, 0]
     assert np.array_equal(run.step([5, 6], [0, 1], [0, 0]).cpu().numpy(), want)
+
+
+def test_largest_position_is_refused(torch, eng):
+    """A position of 2^31 - 1, whose length is no int, is refused like any other outside the table, and leaves the
+    other rows alone."""
+    import _eii
+    run = Run(torch, eng, 16, 16, 2, 32)
+    for pos in ((1 << 31) - 1, (1 << 31) - 2, 512):
+        out = run.step([5, 6], [0, 1], [0, pos], sync=False)
+        with pytest.raises(_eii.EiiError, match="position|length"):
+            run.d.sync(0)
+        run.d.sync(0)
+        assert np.array_equal(out[0].cpu().numpy(), eng.forward(np.array([[5]]))["logits"][0, 0])
