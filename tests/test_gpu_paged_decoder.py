@@ -198,3 +198,45 @@ def test_largest_position_is_refused(torch, eng):
             run.d.sync(0)
         run.d.sync(0)
         assert np.array_equal(out[0].cpu().numpy(), eng.forward(np.array([[5]]))["logits"][0, 0])
+
+
+def paged_equals_forward(torch, e, ids, n_steps=3):
+    """All but the last tokens of two sequences in one step without logits, the rest one by one: the forward pass's rows."""
+    want = [e.forward(x)["logits"][0] for x in ids]
+    run = Run(torch, e, 16, 16, len(ids), max(len(x) for x in ids), seed=2)
+    rows = [(s, t) for s, x in enumerate(ids) for t in range(len(x) - n_steps)]
+    assert run.step([ids[s][t] for s, t in rows], *zip(*rows), logits=False) is None
+    for i in range(n_steps):
+        at = [len(x) - n_steps + i for x in ids]
+        got = run.step([x[t] for x, t in zip(ids, at)], list(range(len(ids))), at).cpu().numpy()
+        for s, t in enumerate(at):
+            assert np.array_equal(got[s], want[s][t]), (s, t)
+
+
+@pytest.mark.parametrize("switch", ["EII_O_FEATURE_MAJOR", "EII_DOWN_ROW_MAJOR", "EII_LOGITS_FEATURE_MAJOR", "EII_NO_NORM_FUSION", "grid"])
+def test_steps_with_the_engines_switches(torch, outlier_model_path, switch, monkeypatch):
+    """The other layouts of the planes that the attention writes and of those behind it, and the narrow residual grid."""
+    import _eii
+    rng = np.random.default_rng(8)
+    if switch != "grid":
+        monkeypatch.setenv(switch, "1")
+    e = _eii.Engine(outlier_model_path, 0)
+    try:
+        if switch == "grid":
+            e.set_residual_grid(rng.integers(0, 4, 30), rng.integers(0, 4, 30))
+        paged_equals_forward(torch, e, [rng.integers(0, V, n) for n in (37, 150)])
+    finally:
+        e.close()
+
+
+def test_step_of_more_rows_than_a_chunk(torch, eng):
+    """A prompt step of more rows than the engine's workspace takes at once."""
+    rng = np.random.default_rng(9)
+    ids = [rng.integers(0, V, 420) for _ in range(160)]
+    run = Run(torch, eng, 64, 16, len(ids), 420)
+    rows = [(s, t) for s in range(len(ids)) for t in range(419)]
+    assert len(rows) > 65536
+    run.step([ids[s][t] for s, t in rows], *zip(*rows), logits=False)
+    got = run.step([x[419] for x in ids], list(range(len(ids))), [419] * len(ids)).cpu().numpy()
+    for s in (0, 78, 79, 80, 159):
+        assert np.array_equal(got[s], eng.forward(ids[s])["logits"][0][419]), s

@@ -713,3 +713,37 @@ def test_sampling_refuses_rows_that_an_int_cannot_step_over(torch, sampler, n):
         sampler.sample(x.data_ptr(), n, 1, x.data_ptr(), x.data_ptr(), stream=st(torch))
     assert e.value.code == _eii.EII_ERR_ARG
     sampler.sync(st(torch))
+
+
+@pytest.mark.parametrize("heads,kv,hd,bits,inp", [(9, 3, 64, 16, 16), (9, 3, 64, 4, 32), (4, 4, 128, 4, 16), (16, 2, 128, 16, 32)])
+@pytest.mark.parametrize("shift", [1, 2, 8, 15, 16, 17, 31, 32, 33, 40, 46, 47, 62])
+def test_append_shifts_and_extremes(torch, heads, kv, hd, bits, inp, shift):
+    """Every kind of shift, for q and k each with the other's neighbour; q, k and v over the whole int16 range, rows
+    of one extreme and rows whose groups hold both (a 4-bit step of 4369); kv_out on a 4-byte boundary."""
+    rng = np.random.default_rng(100 * shift + hd)
+    n = 24
+    c = Cache(torch, rng, heads, kv, hd, 32, bits, [n])
+    x = [rng.integers(-32768, 32768, (n, h, hd)) for h in (heads, kv, kv)]
+    for a in x:
+        a[0], a[1] = -32768, 32767
+        a[2], a[3] = rng.choice([-32768, 32767], a[2].shape), rng.integers(-3, 4, a[3].shape)
+        a[4, :, ::64], a[4, :, 63::64] = -32768, 32767
+    one, zero = np.full((2, hd // 2), 1 << 30, np.int64), np.zeros((2, hd // 2), np.int64)
+    for rope in (c.rope, tuple(np.concatenate(t) for t in ((one, -one, zero, c.rope[0]), (zero, zero, one, c.rope[1])))):
+        import _eii
+        p = _eii.Paged(heads, kv, hd, 32, bits, rope=rope)
+        d = [torch.from_numpy(a.astype(np.int16 if inp == 16 else np.int32)).cuda() for a in x]
+        pos = rng.permutation(n).astype(np.int32)
+        dpos, dseq = torch.from_numpy(pos).cuda(), torch.zeros(n, dtype=torch.int32, device="cuda")
+        other = min(max(shift + rng.choice([-1, 1]), 1), 62)
+        q_out = torch.full((n, heads, hd), 99, dtype=torch.int16, device="cuda")
+        buf = torch.full((n * 2 * kv * hd + 1,), 98, dtype=torch.int32, device="cuda")
+        p.append(c.pages, d[1].data_ptr(), d[2].data_ptr(), n, dpos.data_ptr(), shift, seq_ptr=dseq.data_ptr(), q_ptr=d[0].data_ptr(),
+                 q_out_ptr=q_out.data_ptr(), shift_q=other, in_bits=inp, kv_out_ptr=buf.data_ptr() + 4, stream=st(torch))
+        p.sync(st(torch))
+        wq, wkv = np.zeros((n, heads, hd), np.int64), np.zeros((n, 2, kv, hd), np.int64)
+        osv.append(*x, np.zeros(n, int), pos, c.table, c.k, c.v, rope, other, shift, wq, wkv)
+        assert np.array_equal(q_out.cpu().numpy(), wq)
+        got = buf.cpu().numpy()
+        assert got[0] == 98 and np.array_equal(got[1:].reshape(wkv.shape), wkv)
+        c.check_pools()
