@@ -15,8 +15,10 @@ int fail(int code, const char* fmt, ...);
 #define CK(call)                                                                                      \
     do {                                                                                              \
         cudaError_t e_ = (call);                                                                      \
-        if (e_ != cudaSuccess)                                                                        \
+        if (e_ != cudaSuccess) {                                                                      \
+            cudaGetLastError(); /* reported here, so no later launch is to find it */                 \
             return fail(EII_ERR_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
+        }                                                                                             \
     } while (0)
 #define TRY(...)                         \
     do {                                 \

@@ -60,6 +60,23 @@ int check_ld(const char* name, int64_t ld, int64_t least) {
     return EII_OK;
 }
 
+// Launches in clusters of `cs` blocks and returns this launch's own status (cudaGetLastError may hold an earlier call's).
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kern)(KArgs...), int64_t grid, int block, size_t smem, int cs, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.stream = st;
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cs;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = cs > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 template <int HD, int BITS>
 int launch_append(const AppendParams& ap, int in_bits, int num_sms, cudaStream_t st) {
     // one warp per row, more while that leaves the SMs short of warps and there are heads to share
@@ -75,9 +92,8 @@ int launch_append(const AppendParams& ap, int in_bits, int num_sms, cudaStream_t
     const int vec_in = (in & (4 * e - 1)) == 0;
     const int vec_out = (((reinterpret_cast<uintptr_t>(ap.q_out) | static_cast<uintptr_t>(ap.ldqo * 2)) & 7) == 0) |
                         ((reinterpret_cast<uintptr_t>(ap.kv_out) & 15) == 0) << 1;
-    if (in_bits == 16) k_paged_append<HD, BITS, int16_t><<<(unsigned)blocks, 256, 0, st>>>(ap, wpr, vec_in, vec_out);
-    else k_paged_append<HD, BITS, int32_t><<<(unsigned)blocks, 256, 0, st>>>(ap, wpr, vec_in, vec_out);
-    CK(cudaGetLastError());
+    if (in_bits == 16) CK(launch(k_paged_append<HD, BITS, int16_t>, blocks, 256, 0, 1, st, ap, wpr, vec_in, vec_out));
+    else CK(launch(k_paged_append<HD, BITS, int32_t>, blocks, 256, 0, 1, st, ap, wpr, vec_in, vec_out));
     return EII_OK;
 }
 
@@ -152,25 +168,14 @@ int launch_attention_nh(const eii_paged* p, const PagedAttnParams& ap, cudaStrea
     if (items > INT32_MAX / PATTN_MAX_CLUSTER) return fail(EII_ERR_ARG, "n_rows %d is too large", ap.n_rows);
     AttnShape s = attn_shape(items, tiles, NH, HD, BITS, p->num_sms);
     if (s.warp) {
-        k_paged_attention<HD, BITS, NH, true><<<static_cast<unsigned>((items + s.warps - 1) / s.warps), 32 * s.warps,
-                                               C::smem_warp(s.warps, tiles * 32), st>>>(ap, 1, tiles * 32, static_cast<int>(items));
-        CK(cudaGetLastError());
+        CK(launch(k_paged_attention<HD, BITS, NH, true>, (items + s.warps - 1) / s.warps, 32 * s.warps,
+                  C::smem_warp(s.warps, tiles * 32), 1, st, ap, 1, tiles * 32, static_cast<int>(items)));
         return EII_OK;
     }
     const int part = (tiles + s.cs - 1) / s.cs * 32;
     if (C::smem_block(s.warps, part) > kSmemOptin) s.warps = 8;
-    cudaLaunchConfig_t cfg{};
-    cfg.stream = st;
-    cfg.blockDim = dim3(32 * s.warps);
-    cfg.gridDim = dim3(static_cast<unsigned>(items * s.cs));
-    cfg.dynamicSmemBytes = C::smem_block(s.warps, part);
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = s.cs;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = s.cs > 1 ? 1 : 0;
-    CK(cudaLaunchKernelEx(&cfg, k_paged_attention<HD, BITS, NH, false>, ap, s.cs, part, static_cast<int>(items)));
+    CK(launch(k_paged_attention<HD, BITS, NH, false>, items * s.cs, 32 * s.warps, C::smem_block(s.warps, part), s.cs, st, ap,
+              s.cs, part, static_cast<int>(items)));
     return EII_OK;
 }
 

@@ -747,3 +747,37 @@ def test_append_shifts_and_extremes(torch, heads, kv, hd, bits, inp, shift):
         got = buf.cpu().numpy()
         assert got[0] == 98 and np.array_equal(got[1:].reshape(wkv.shape), wkv)
         c.check_pools()
+
+
+def test_calls_after_a_failed_allocation(torch, base_model_path):
+    """A decoder whose pools do not fit is refused, and the calls that follow are not blamed for it."""
+    import _eii
+    rng = np.random.default_rng(14)
+    lens = [40] * 500
+    e = _eii.Engine(base_model_path, 0)
+    try:
+        c = Cache(torch, rng, 9, 3, 64, 16, 16, lens)
+        c.fill(rng, lens[:0])
+        x = [rng.integers(-32768, 32768, (2, h, 64)) for h in (9, 3, 3)]
+        d = [torch.from_numpy(a.astype(np.int16)).cuda() for a in x]
+        pos, seq = np.array([39, 8], np.int32), np.array([0, 1], np.int32)
+        dpos = torch.from_numpy(pos).cuda()
+
+        def refused():
+            with pytest.raises(_eii.EiiError) as err:
+                _eii.PagedDecoder(e, 1024, 16, (1 << 31) - 1)
+            assert err.value.code == _eii.EII_ERR_CUDA
+        refused()
+        c.p.append(c.pages, d[1].data_ptr(), d[2].data_ptr(), 2, dpos.data_ptr(), 30, stream=st(torch))
+        c.p.sync(st(torch))
+        osv.append(None, x[1], x[2], seq, pos, c.table, c.k, c.v, c.rope, 30, 30, None, np.zeros((2, 2, 3, 64), np.int64))
+        c.check_pools()
+        refused()  # (500 short rows: one warp per item)
+        check_attention(torch, c, rng, None, [1] * 500, 40)
+        refused()
+        check_attention(torch, c, rng, [0], [40], 40)
+        a, W, one = rng.integers(-100, 100, (4, 32)), rng.integers(-100, 100, (16, 32)), np.ones(16, np.int64)
+        refused()
+        assert np.array_equal(e.linear(a, 16, W, one, one * 8, 0, 0, 32)[1], a @ W.T)
+    finally:
+        e.close()
