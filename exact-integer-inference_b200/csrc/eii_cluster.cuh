@@ -39,7 +39,9 @@ __device__ __forceinline__ int64_t ld_remote64(uint32_t a) {
     asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
     return v;
 }
-// Sum of a non-negative v < 2^47 over the warp, in pieces of 24 and 23 bits.
+// Sum of a non-negative v over the warp, in pieces of 24 bits and the rest.  Exact where every lane's v (one thread's,
+// warp's or block's part) is below 2^51, so that 32 upper pieces stay in 32 bits; the parts here are below
+// 2^47, their sum may be more: 2^18 weights of 2^30 make 2^48.
 __device__ __forceinline__ uint64_t warp_sum47(uint64_t v) {
     const uint32_t lo = __reduce_add_sync(~0u, static_cast<uint32_t>(v) & 0xFFFFFFu);
     const uint32_t hi = __reduce_add_sync(~0u, static_cast<uint32_t>(v >> 24));

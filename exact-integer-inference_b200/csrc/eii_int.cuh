@@ -29,7 +29,7 @@ __device__ __forceinline__ uint8_t plane_byte(int64_t a, int p) {
     return static_cast<uint8_t>(static_cast<uint64_t>(a >> (8 * p)) & 0xFFu);
 }
 
-// Row-blocked planes.  // Activation byte planes read by the GEMMs through the row-blocked layout
+// Activation byte planes that the GEMMs read through the row-blocked layout
 // [P][ceil(M/128)][K/16][128 rows][16 bytes]: byte k of row r of a plane sits at blocked_off(r, k, K),
 // so 32 consecutive rows x 16 bytes are 512 contiguous bytes (coalesced epilogue stores) and a GEMM
 // reads a 128-row x 128-byte K block as eight 2 KB runs (see map_blocked on the host).

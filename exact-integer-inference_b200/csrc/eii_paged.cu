@@ -26,7 +26,7 @@ int64_t slab_bytes(const eii_paged* p) {
     return static_cast<int64_t>(paged_row_bytes(p->hd, p->bits)) << p->page_shift;
 }
 
-int check_pages(const eii_paged* p, const eii_pages* pg) {
+int check_pages(const eii_pages* pg) {
     if (!pg) return fail(EII_ERR_ARG, "pages is null");
     if (!pg->k_pool || !pg->v_pool || !pg->table) return fail(EII_ERR_ARG, "a pool or the page table is null");
     if ((reinterpret_cast<uintptr_t>(pg->k_pool) | reinterpret_cast<uintptr_t>(pg->v_pool)) & 15)
@@ -36,7 +36,6 @@ int check_pages(const eii_paged* p, const eii_pages* pg) {
         return fail(EII_ERR_ARG, "n_pages must be in [1, 2^31) (got %lld)", (long long)pg->n_pages);
     if (pg->n_seq < 1) return fail(EII_ERR_ARG, "n_seq must be >= 1 (got %d)", pg->n_seq);
     if (pg->ld_table < 1) return fail(EII_ERR_ARG, "ld_table must be >= 1 (got %lld)", (long long)pg->ld_table);
-    (void)p;
     return EII_OK;
 }
 
@@ -298,7 +297,7 @@ int eii_paged_append(eii_paged* p, const eii_pages* pages, const void* q, int64_
     if (!p) return fail(EII_ERR_ARG, "cache is null");
     if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
     if (n_rows == 0) return EII_OK;
-    TRY(check_pages(p, pages));
+    TRY(check_pages(pages));
     if (!k || !v || !pos) return fail(EII_ERR_ARG, "k, v or pos is null");
     if (!q != !q_out) return fail(EII_ERR_ARG, "q and q_out come together");
     if (in_bits != 16 && in_bits != 32) return fail(EII_ERR_ARG, "in_bits must be 16 or 32 (got %d)", in_bits);
@@ -342,7 +341,7 @@ int eii_paged_attention(eii_paged* p, const eii_pages* pages, const int16_t* q, 
     if (!p) return fail(EII_ERR_ARG, "cache is null");
     if (n_rows < 0) return fail(EII_ERR_ARG, "n_rows must be >= 0 (got %d)", n_rows);
     if (n_rows == 0) return EII_OK;
-    TRY(check_pages(p, pages));
+    TRY(check_pages(pages));
     if (!q || !len || !ctx) return fail(EII_ERR_ARG, "q, len or ctx is null");
     if (!seq && n_rows > pages->n_seq)
         return fail(EII_ERR_ARG, "%d rows without sequence indices but %d sequences", n_rows, pages->n_seq);

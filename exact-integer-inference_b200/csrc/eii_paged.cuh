@@ -129,8 +129,9 @@ __device__ __forceinline__ uint32_t quantise4(int32_t (&x)[N], uint32_t (&nib)[N
 // `wpr` warps per row take turns at its steps: four (two) heads of q, then of k, then of v, HD / 8 lanes each; the
 // row's position, page and each lane's four cosines and sines stay in registers.  16-byte loads of int32
 // inputs, 8-byte ones of int16, element by element where alignment does not allow them.  65536 rows of 15
-// heads to 16 bits take 100 us (0.73 of the copy rate), one warp per head and row 226; the rotation's integer
-// instructions bound it.
+// heads to 16 bits take 100 us (0.73 of the copy rate), one warp per head and row 226.  Bound by the latency of its
+// loads, for which a warp waits more than half of its time, with the 34 warps that an SM holds at 48 registers (issue
+// slots 52% busy, integer pipe 39%); 20011 rows of 48 heads of 128 to 4 bits 152 us (0.61), 28 warps at 62 (49%, 39%).
 template <int HD, int BITS, typename T>
 __global__ void __launch_bounds__(256) k_paged_append(const AppendParams p, const int wpr, const int vec_in, const int vec_out) {
     constexpr int LANES = AppendLanes<HD>::LANES, HEADS = AppendLanes<HD>::HEADS, HALF = HD / 2;
@@ -402,8 +403,9 @@ __device__ __forceinline__ uint32_t prob_exact(uint32_t q, uint32_t e, int pb, u
 //     words are transposed in registers), dimensions are columns.  4 bits: W = P m <= 2^19 4369 < 2^32, and
 //     sum_j P_j z_j apart; 16 bits: W = P, the bytes of v in separate columns.
 // An item with fewer heads than NH computes the absent ones from zeros and drops them.
-// Bound by instruction latency and issue, not by memory: a tile of 32 keys and three heads is about 700 instructions
-// of its warp.  4096 sequences of 128 keys at 16 bits take 88 us (0.61 of the copy rate; 227 without the ring and
+// Bound by instruction latency, not by memory: a tile of 32 keys and three heads is about 700 instructions of its warp,
+// mostly in one dependent chain, and 7 to 16 warps on an SM (registers, ring; for want of items) keep 37 to 53% of the
+// issue slots busy.  4096 sequences of 128 keys at 16 bits take 88 us (0.61 of the copy rate; 227 without the ring and
 // with four warps per item), 512 of up to 512 keys at 4 bits 27, one of 65521 at 4 bits 24.
 // The bounds give a thread 128 registers; with room for 24 warps per SM instead of 16 (80 registers at 4 bits and
 // head_dim 64) 512 of up to 512 keys took 32.

@@ -21,7 +21,7 @@ namespace eii {
 constexpr uint32_t SAMPLE_C1 = 744163075, SAMPLE_C2 = 257059888, SAMPLE_C3 = 57045411, SAMPLE_C4 = 7277686;
 constexpr int64_t SAMPLE_LOG2E_Q24 = 24204406;
 constexpr int32_t SAMPLE_MASKED = INT32_MIN;
-constexpr int SAMPLE_MAX_VOCAB = 262144;  // 2^30 x 2^18 weights: sums stay below 2^48
+constexpr int SAMPLE_MAX_VOCAB = 262144;  // 2^18 weights of at most 2^30: sums are at most 2^48
 constexpr int32_t SAMPLE_MAX_INV_TEMP = 1 << 22;
 constexpr int SAMPLE_MAX_ROWS = 1 << 30;
 
@@ -143,10 +143,12 @@ struct SampleShared {
 };
 static_assert(SAMPLE_MAX_CHUNKS * 16 * SAMPLE_THREADS + sizeof(SampleShared) <= 227 * 1024, "shared memory");
 
-// Bound by the integer pipe: of 49,000 cycles of a row of 49152 (top-p) the weights take about 14,000, each of two
-// passes 5,000, the sample 6,000, the list and its search 12,000.  4096 such rows take 855 us, 0.94 TB/s of the 6.5
-// that a copy reaches.  The weights in registers instead of shared memory (96 per thread, 512 threads) took 1,600
-// us: unrolled code and spills.
+// Bound by one row at a time on an SM (its weights fill the shared memory): no other block has work while this one waits
+// at its barriers and searches its list.  Of 49,000 cycles of a row of 49152 (top-p) the weights take about 14,000, each
+// of two passes 5,000, the sample 6,000, the list and its search 12,000; over all of them 63% of the issue slots
+// and 55% of the integer pipe are busy, with a small top-k 49% and 32%.  4096 such rows take 858 us, 0.94 TB/s of the
+// 6.5 that a copy reaches.  The weights in registers instead of shared memory (96 per thread, 512 threads) took
+// 1,600 us: unrolled code and spills.
 __global__ void __launch_bounds__(SAMPLE_THREADS, 1) k_sample(const SampleParams p, const int cs, const int ch, const int aligned) {
     extern __shared__ __align__(16) uint8_t smem[];
     SampleShared& sh = *reinterpret_cast<SampleShared*>(smem + ch * 16 * SAMPLE_THREADS);
